@@ -17,6 +17,7 @@
 #include <vector>
 
 #include "../../include/fisr.h"
+#include "host_util.h"
 // FISR_DIAG builds (scripts/gpu_*.sh, lib.build(diag=True) -> build_ab/libfisr_hip_diag.so) add what the shipped library
 // must not have: environment switches that change which kernel runs (FISR_WINO_VARIANT, FISR_CONV_MR, FISR_HEAD_VALU,
 // FISR_CONV_HEAD16), the two superseded Winograd kernels, the compile-time ablations (-DFISR_ABL / -DFISR_WABL) and the
@@ -103,6 +104,10 @@ int fail(fisr_ctx* ctx, int code, const std::string& msg) {
   return code;
 }
 
+}  // namespace
+int fisr::set_error(int code, const std::string& msg) { return fail(nullptr, code, msg); }
+namespace {
+
 #define HIP_OK(ctx, expr)                                                                   \
   do {                                                                                      \
     hipError_t e_ = (expr);                                                                 \
@@ -112,32 +117,8 @@ int fail(fisr_ctx* ctx, int code, const std::string& msg) {
 
 inline int round_up(int v, int m) { return (v + m - 1) / m * m; }
 
-// Every entry point that launches work selects the device the work belongs to and restores the caller's
-// current device on return (a host may drive several GPUs, one ctx each, from one thread; torch's notion of
-// the current device must not change behind its back).
-struct DeviceGuard {
-  int prev = -1;
-  bool switched = false;
-  hipError_t err = hipSuccess;
-  explicit DeviceGuard(int dev) {
-    if (dev < 0) return;
-    err = hipGetDevice(&prev);
-    if (err == hipSuccess && prev != dev) { err = hipSetDevice(dev); switched = err == hipSuccess; }
-  }
-  ~DeviceGuard() { if (switched) (void)hipSetDevice(prev); }
-};
-// Device that owns a device pointer (glue entry points have no ctx: the output tensor decides); -1 if unknown.
-inline int device_of(const void* p) {
-  hipPointerAttribute_t a;
-  if (!p || hipPointerGetAttributes(&a, p) != hipSuccess) { (void)hipGetLastError(); return -1; }
-  return a.type == hipMemoryTypeDevice || a.type == hipMemoryTypeManaged ? a.device : -1;
-}
 inline int ilog2(int v) { int k = 0; while ((1 << (k + 1)) <= v) ++k; return k; }
 inline bool is_pow2(int v) { return v > 0 && (v & (v - 1)) == 0; }
-inline int grid_for(size_t work, int block = 256) {
-  size_t g = (work + block - 1) / block;
-  return (int)std::min<size_t>(std::max<size_t>(g, 1), 256 * 16);
-}
 
 // The 138 conv names with their channel counts (reference ops.py:48-76, FISRnet.py:83-106;
 // same order as fisr_amd/weights.py conv_specs()).

@@ -9,7 +9,8 @@ from __future__ import annotations
 import ctypes
 import os
 import subprocess
-from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int64, c_size_t, c_uint8, c_void_p
+import tempfile
+from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int64, c_size_t, c_uint64, c_uint8, c_void_p
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 _ROOT = os.path.dirname(_PKG)
@@ -17,6 +18,8 @@ SO_PATH = os.environ.get("FISR_HIP_SO") or os.path.join(_PKG, "libfisr_hip.so") 
 CSRC = os.path.join(_PKG, "csrc")
 
 PREC_F32, PREC_F16, PREC_BF16X3, PREC_F16F8, PREC_F32W, PREC_MIXED, PREC_F16R, PREC_MIXEDR, PREC_F32W4, PREC_F16F8R = 0, 1, 2, 3, 4, 5, 6, 7, 8, 9
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2
+ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU = 0, 1, 2, 3
 CONV_RELU_IN, CONV_RELU_OUT, CONV_D2S, CONV_UP2_IN = 1, 2, 4, 8
 
 EXPORTS = [
@@ -35,6 +38,7 @@ EXPORTS = [
     "fisr_train_packed_bytes", "fisr_train_pack", "fisr_train_wino_bytes", "fisr_train_pack_wino", "fisr_train_pack_all", "fisr_train_conv3x3", "fisr_train_wgrad", "fisr_train_bgrad",
     "fisr_train_relu_bwd", "fisr_train_axpy", "fisr_train_maxpool2_bwd", "fisr_train_upsample2_bwd", "fisr_train_s2d",
     "fisr_train_copy_channels", "fisr_train_loss", "fisr_train_adam",
+    "fisr_train_groupnorm_workspace_bytes", "fisr_train_groupnorm", "fisr_train_groupnorm_bwd", "fisr_train_dropout",
 ]
 COMM_ID_BYTES = 128
 
@@ -83,13 +87,18 @@ def build(force: bool = False, verbose: bool = False, diag: bool = False, define
     if not diag and not out and not force and not needs_build():
         return SO_PATH
     os.makedirs(os.path.dirname(target), exist_ok=True)
-    cmd = [hipcc_path(), "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-           "-Wl,--version-script=" + os.path.join(CSRC, "exports.map"),
-           f'-DFISR_SRC_HASH="{source_hash()}"'] + (["-DFISR_DIAG"] if diag else []) + [f"-D{d}" for d in defines] + \
-          ["-o", target, os.path.join(CSRC, "fisr_api.hip")]
-    if verbose:
-        print(" ".join(cmd))
-    subprocess.check_call(cmd)
+    flags = [hipcc_path(), "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden"]
+    with tempfile.TemporaryDirectory() as d:
+        # fisr_api.hip's Winograd kernels write packed float32 instructions by hand; everything else is compiled without them
+        norm_o = os.path.join(d, "fisr_norm.o")
+        norm = flags + ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-c", "-o", norm_o, os.path.join(CSRC, "fisr_norm.hip")]
+        cmd = flags + ["-shared", "-Wl,--version-script=" + os.path.join(CSRC, "exports.map"),
+                       f'-DFISR_SRC_HASH="{source_hash()}"'] + (["-DFISR_DIAG"] if diag else []) + [f"-D{x}" for x in defines] + \
+              ["-o", target, os.path.join(CSRC, "fisr_api.hip"), "-x", "none", norm_o]
+        if verbose:
+            print(" ".join(norm), " ".join(cmd), sep="\n")
+        subprocess.check_call(norm)
+        subprocess.check_call(cmd)
     return target
 
 
@@ -99,6 +108,11 @@ MAX_SRC_ITEMS = 16          # FISR_MAX_SRC_ITEMS (include/fisr.h)
 class SrcItem(ctypes.Structure):
     """fisr_src_item (include/fisr.h): one tile of one window for fisr_forward_frames."""
     _fields_ = [("frames", c_void_p * 3), ("flows", c_void_p * 4), ("warps", c_void_p * 4), ("y0", c_int), ("x0", c_int)]
+
+
+class DropoutDesc(ctypes.Structure):
+    """fisr_dropout (include/fisr.h)."""
+    _fields_ = [("p", c_double), ("seed", c_uint64), ("offset", c_uint64), ("d_counter", c_void_p)]
 
 
 _lib = None
@@ -198,6 +212,11 @@ def lib():
     L.fisr_train_copy_channels.argtypes = [vp, c_int, c_int, vp, c_int, c_int, c_int, c_size_t, c_int, vp]
     L.fisr_train_loss.argtypes = [POINTER(vp), vp, POINTER(vp), vp, c_size_t, POINTER(c_float), vp]
     L.fisr_train_adam.argtypes = [vp, vp, vp, vp, c_size_t, c_float, c_float, c_float, c_float, vp]
+    L.fisr_train_groupnorm_workspace_bytes.argtypes = [c_int] * 6
+    L.fisr_train_groupnorm_workspace_bytes.restype = c_size_t
+    L.fisr_train_groupnorm.argtypes = [vp, c_int, vp, vp, vp, c_int, vp] + [c_int] * 5 + [c_float, c_int, POINTER(DropoutDesc), c_int, vp, c_size_t, vp]
+    L.fisr_train_groupnorm_bwd.argtypes = [vp, c_int, vp, c_int, vp, vp, vp, vp, c_int, vp, vp] + [c_int] * 7 + [POINTER(DropoutDesc), c_int, vp, c_size_t, vp]
+    L.fisr_train_dropout.argtypes = [vp, vp, vp, c_size_t, POINTER(DropoutDesc), c_int, vp]
     _lib = L
     return L
 

@@ -378,6 +378,40 @@ FISR_API int fisr_train_loss(const float* const* pred4, const float* gt, float* 
 FISR_API int fisr_train_adam(float* w, const float* g, float* m, float* v, size_t count, float lr_t, float b1, float b2,
                     float eps, void* stream);
 
+/* ---- normalisation and dropout (training ops beside those above; the reference has neither) ----
+ * Tensors are channels last, [n,h,w,c] with a pixel stride of *_cs >= c elements (a range of a wider buffer's channels; the pixels of
+ * an image and the images follow each other without gaps); `type` is the type of all of a call's tensors, the parameters, statistics
+ * and parameter gradients are float32.  Arithmetic is float32 throughout, outputs are rounded once.  Results are the same bits on
+ * every call (no atomics).  Nothing is kept between calls; calls that run at the same time need workspaces of their own. */
+enum { FISR_TYPE_F32 = 0, FISR_TYPE_F16 = 1, FISR_TYPE_BF16 = 2 };
+enum { FISR_ACT_NONE = 0, FISR_ACT_RELU = 1, FISR_ACT_SILU = 2, FISR_ACT_GELU = 3 /* z * Phi(z) */ };
+/* Dropout whose mask is a function of (seed, offset, element) and is never stored: element i of the dense tensor [n,h,w,c] is dropped
+ * where the 16-bit number i % 8 of block i / 8 of Philox4x32-7 (counter words: i / 8 low, high, offset low, high; key: seed low, high) is
+ * below t = round(65536 p); the others are multiplied by 65536 / (65536 - t).  p = 1 drops everything.  Dropped elements are zero
+ * whatever they held.  The backward pass is given the same struct.  Use another offset for every call that should draw another mask.
+ * d_counter (nullable): a device uint64 that is added to offset when the kernel runs, so that a captured graph draws a new mask on
+ * every replay if the counter is advanced between them. */
+typedef struct fisr_dropout {
+  double p;
+  uint64_t seed, offset;
+  const uint64_t* d_counter;
+} fisr_dropout;
+/* y = drop(act((x - mean) * rstd * gamma + beta)), mean and rstd = 1 / sqrt(var + eps) over the pixels and the c / groups channels of
+ * a group.  gamma, beta [c] (nullable: ones, zeros); mean_rstd [2][n][groups]: means, then rstd (written; the backward pass reads it);
+ * drop nullable; y may be x.  workspace: caller-owned, 16-byte aligned, of fisr_train_groupnorm_workspace_bytes (0: bad shape). */
+FISR_API size_t fisr_train_groupnorm_workspace_bytes(int n, int h, int w, int c, int groups, int backward);
+FISR_API int fisr_train_groupnorm(const void* x, int x_cs, const float* gamma, const float* beta, void* y, int y_cs, float* mean_rstd, int n,
+                     int h, int w, int c, int groups, float eps, int act, const fisr_dropout* drop, int type, void* workspace,
+                     size_t workspace_bytes, void* stream);
+/* its gradients from the forward pass' x and mean_rstd: dx (may be dy, not x), and dgamma, dbeta [c] (nullable), overwritten or, with
+ * accumulate != 0, added to */
+FISR_API int fisr_train_groupnorm_bwd(const void* x, int x_cs, const void* dy, int dy_cs, const float* gamma, const float* beta,
+                     const float* mean_rstd, void* dx, int dx_cs, float* dgamma, float* dbeta, int accumulate, int n, int h, int w, int c,
+                     int groups, int act, const fisr_dropout* drop, int type, void* workspace, size_t workspace_bytes, void* stream);
+/* y = drop(x) [+ residual] on `count` elements (residual nullable; y may be x or residual).  The gradient with respect to x is the same
+ * call on dy without a residual. */
+FISR_API int fisr_train_dropout(const void* x, const void* residual, void* y, size_t count, const fisr_dropout* drop, int type, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

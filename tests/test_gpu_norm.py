@@ -1,0 +1,373 @@
+"""Group normalisation with an activation and counter-based dropout (fisr_amd/norm.py) against the float64 oracle.
+
+Tolerances.  U = half a step of the tensors' type (2^-24, 2^-11, 2^-8) rounds each output once; everything before it is float32, E = 2^-24.
+A thread sums at most CHAIN = 256 values one after the other at the sizes below (chunks of at most 8192 elements + 256 threads' rows, or
+tensors of that size), so a mean is off by at most K E max|x| and a sum by K E sum|terms| with K = CHAIN + 32 for the joins; what one
+rounding adds to a value v is E |v|.  With X = max|x| of an image:
+  mean: K E X;  rstd: relative (K + 2 X rstd) E (the squared deviations' own roundings, each |x - mean| to E X)
+  z = (x - mean) rstd gamma + beta: Z = |gamma| rstd K E X + |gamma xh| (K + 2 X rstd + 4) E + E |z|
+  y: 1.13 Z (the activations' largest slope) + 8 E |y| (activation) + 2e-7 |z| (its approximations' absolute error) + U |y|
+  dz = dy act'(z): |dy| (1.0 Z (their largest curvature) + 1e-6);  sums A, B: sum of these + K E sum |dz|, with |xh| and its error for B
+  dx: rstd (|gamma| dz's + (|gamma| A's / M + |xh| |gamma| B's / M summed over the group) + 8 E of each term) + U |dx|, and what xh's error
+  times S2 gives."""
+import numpy as np
+import pytest
+
+import fisr_norm_oracle as no
+
+pytestmark = pytest.mark.gpu
+E, K = 2.0 ** -24, 288
+HALF = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}
+TINY = {"f32": 2.0 ** -126, "f16": 2.0 ** -24, "bf16": 2.0 ** -126}      # a step of the smallest numbers: float16 has subnormals in range
+
+
+@pytest.fixture(scope="module")
+def env():
+    import torch
+    if not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+    from fisr_amd import norm
+    return torch, norm
+
+
+def _type(torch, t):
+    return {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[t]
+
+
+def _to(torch, a, t):
+    return torch.from_numpy(np.ascontiguousarray(a, np.float32)).to("cuda:0", _type(torch, t))
+
+
+def _np(t):
+    return t.detach().double().cpu().numpy()
+
+
+def _inputs(torch, n, h, w, c, t, seed, shift=0.5):
+    """x, dy (as the type holds them, in float64 too), gamma, beta."""
+    r = np.random.default_rng(seed)
+    x = r.standard_normal((n, h, w, c)) * (0.5 + r.random(c)) + shift + r.standard_normal(c)
+    dy = r.standard_normal((n, h, w, c))
+    x, dy = (_to(torch, v, t) for v in (x, dy))
+    gamma, beta = (_to(torch, v, "f32") for v in (1 + 0.2 * r.standard_normal(c), 0.2 * r.standard_normal(c)))
+    return x, dy, gamma, beta
+
+
+def _bounds(x, groups, gamma, beta, eps, act, fac, half, tiny):
+    """(y, mean, rstd, their bounds, z's bound, xh's bound) by the docstring's arithmetic."""
+    y, mean, rstd, z, xh = no.forward(x, groups, gamma, beta, eps, act, fac)
+    c = x.shape[3]
+    X = np.abs(x).max(axis=(1, 2, 3))[:, None]
+    emean = K * E * X + 0 * mean
+    erstd = (K + 2 * X * rstd) * E
+    exh = no.per_channel(rstd * emean, c) + np.abs(xh) * (no.per_channel(erstd, c) + 4 * E)
+    ez = np.abs(gamma) * exh + E * np.abs(z)
+    ey = fac * (1.13 * ez + 8 * E * np.abs(act_abs(z, act)) + 2e-7 * np.abs(z)) + half * np.abs(y) + tiny
+    return y, mean, rstd, ey, emean + E * np.abs(mean), (erstd + E) * rstd, ez, exh
+
+
+def act_abs(z, act):
+    return np.abs(no.act(z, act))
+
+
+def _within(got, want, bound, what):
+    bad = ~(np.abs(got - want) <= bound)
+    assert not bad.any(), (what, int(bad.sum()), got[bad][:4], want[bad][:4], np.broadcast_to(bound, bad.shape)[bad][:4])
+
+
+SHAPES = [
+    # (n, h, w, c, groups)
+    (1, 1, 1, 1, 1), (1, 1, 1, 8, 1), (2, 1, 1, 64, 8), (3, 1, 2, 2, 2), (1, 1, 7, 6, 3), (2, 3, 3, 512, 32), (4, 6, 6, 256, 32), (1, 5, 9, 29, 29),
+    (2, 13, 11, 29, 1), (2, 17, 9, 36, 4), (1, 24, 24, 64, 64), (3, 12, 12, 512, 1), (2, 19, 23, 40, 5), (2, 9, 7, 12, 2), (1, 3, 2, 600, 4),
+    (1, 2, 3, 4104, 8), (2, 2, 2, 2060, 4), (1, 1, 3, 1027, 13), (37, 3, 5, 16, 16), (2, 96, 96, 64, 8), (1, 130, 70, 8, 2), (1, 191, 67, 3, 1),
+    (5, 31, 33, 24, 8), (300, 2, 2, 8, 4),
+]
+KINDS = [("f32", "none", 0.0), ("f32", "silu", 0.25), ("f16", "gelu", 0.0), ("f16", "relu", 0.1), ("bf16", "silu", 0.0), ("bf16", "gelu", 0.5), ("f32", "relu", 0.0),
+         ("f32", "gelu", 0.1)]
+
+
+@pytest.mark.parametrize("t,act,p", KINDS)
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s)))
+def test_group_norm_and_gradients_vs_oracle(env, shape, t, act, p):
+    torch, norm = env
+    n, h, w, c, groups = shape
+    x, dy, gamma, beta = _inputs(torch, n, h, w, c, t, n * 1000 + h * 10 + c)
+    x64, dy64, g64, b64 = map(_np, (x, dy, gamma, beta))
+    seed, offset = 0xFEDCBA9876543210, (1 << 40) + 77
+    drop = norm.Dropout(p, seed, offset) if p else None
+    fac = no.drop_factor(x64.shape, p, seed, offset) if p else np.ones_like(x64)
+    y64, mean, rstd, ey, emean, erstd, ez, exh = _bounds(x64, groups, g64, b64, 1e-5, act, fac, HALF[t], TINY[t])
+    y, stats = norm.group_norm(x, groups, gamma, beta, act=act, dropout=drop)
+    got = _np(stats)
+    _within(got[0], mean, emean, "mean")
+    _within(got[1], rstd, erstd, "rstd")
+    _within(_np(y), y64, ey, "y")
+    # ---- gradients (relu: no gradient comes in where rounding decides the sign of z)
+    if act == "relu":
+        dy64 = np.where(np.abs(no.forward(x64, groups, g64, b64, 1e-5, act)[3]) <= ez, 0.0, dy64)
+        dy = _to(torch, dy64, t)
+    m = h * w * (c // groups)
+    dx64, dg64, db64 = no.backward(dy64, x64, groups, g64, b64, 1e-5, act, fac)
+    z, xh = no.forward(x64, groups, g64, b64, 1e-5, act)[3:5]
+    dz = np.abs(dy64 * fac * no.act_grad(z, act))
+    curve = 0.0 if act in ("none", "relu") else 1.0
+    edz = np.abs(dy64) * fac * (curve * ez + 1e-6)
+    ta, tb = edz + K * E * dz, (edz + K * E * dz) * np.abs(xh) + dz * exh            # errors of the terms of A, B, with the sums' own
+    grp = lambda v: no.per_channel((v.sum(axis=(1, 2)) * np.abs(g64)).reshape(n, groups, -1).sum(2) / m, c)  # noqa: E731
+    rs = no.per_channel(rstd, c)
+    s2 = grp(dz * np.abs(xh))
+    edx = rs * (np.abs(g64) * (edz + 8 * E * dz) + grp(ta) + np.abs(xh) * grp(tb) + exh * s2 + 8 * E * (grp(dz) + np.abs(xh) * s2)) + HALF[t] * np.abs(dx64) + TINY[t]
+    edx = edx + no.per_channel(erstd, c) / rs * (np.abs(dx64) + rs * (np.abs(g64) * dz + grp(dz) + np.abs(xh) * s2))
+    dx, dg, db = norm.group_norm_backward(dy, x, stats, groups, gamma, beta, act=act, dropout=drop)
+    _within(_np(db), db64, ta.sum(axis=(0, 1, 2)) + E * np.abs(db64), "dbeta")
+    _within(_np(dg), dg64, tb.sum(axis=(0, 1, 2)) + E * np.abs(dg64), "dgamma")
+    _within(_np(dx), dx64, edx, "dx")
+
+
+def test_mean_far_from_the_values_spread(env):
+    """Values around 4096 with a spread of 1: a sum of squares about zero would lose all of it.  The bound of the docstring holds with
+    X rstd = 4100."""
+    torch, norm = env
+    x, _, gamma, beta = _inputs(torch, 2, 40, 36, 32, "f32", 5, shift=4096.0)
+    x[:, 0, 0] = 0.0                                       # the first pixel is far from all others
+    x64, g64, b64 = map(_np, (x, gamma, beta))
+    y64, mean, rstd, ey, emean, erstd, _, _ = _bounds(x64, 4, g64, b64, 1e-5, "none", 1.0, E, 0.0)
+    y, stats = norm.group_norm(x, 4, gamma, beta)
+    _within(_np(stats)[1], rstd, erstd, "rstd")
+    _within(_np(y), y64, ey, "y")
+
+
+def test_without_parameters_and_accumulated(env):
+    torch, norm = env
+    x, dy, _, _ = _inputs(torch, 2, 9, 7, 24, "f32", 8)
+    one, zero = torch.ones(24, device="cuda:0"), torch.zeros(24, device="cuda:0")
+    y, st = norm.group_norm(x, 3, act="silu")
+    y1, st1 = norm.group_norm(x, 3, one, zero, act="silu")
+    assert torch.equal(y, y1) and torch.equal(st, st1)
+    a = norm.group_norm_backward(dy, x, st, 3, act="silu")
+    b = norm.group_norm_backward(dy, x, st, 3, one, zero, act="silu")
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    dg, db = torch.full((24,), 2.0, device="cuda:0"), torch.full((24,), -3.0, device="cuda:0")
+    norm.group_norm_backward(dy, x, st, 3, act="silu", dgamma=dg, dbeta=db, accumulate=True)
+    assert torch.allclose(dg, a[1] + 2.0, rtol=0, atol=float(4 * E * (a[1].abs().max() + 2))) and torch.allclose(db, a[2] - 3.0, rtol=0, atol=float(4 * E * (a[2].abs().max() + 3)))
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("c,lo,hi", [(24, 0, 8), (24, 8, 24), (40, 4, 20), (40, 1, 13), (13, 2, 12)])
+def test_channel_ranges_of_wider_buffers(env, t, c, lo, hi):
+    """Strided pixels, bases that fit no vector load: the dense call's results, and nothing written beside the range."""
+    torch, norm = env
+    x, dy, gamma, beta = _inputs(torch, 2, 11, 13, c, t, 4)
+    k = hi - lo
+    g, b = gamma[:k].clone(), beta[:k].clone()
+    xs, dys = x[..., lo:hi], dy[..., lo:hi]
+    drop = norm.Dropout(0.3, 5, 6)
+    y0, st0 = norm.group_norm(xs.contiguous(), 2, g, b, act="gelu", dropout=drop)
+    out = torch.full_like(x, 7.0)
+    y1, st1 = norm.group_norm(xs, 2, g, b, act="gelu", dropout=drop, out=out[..., lo:hi])
+    tol = 3 * HALF[t]                                       # another vector width sums in another order
+    assert torch.allclose(st0, st1, rtol=K * E, atol=K * E)
+    assert torch.allclose(y0.double(), y1.double(), rtol=tol, atol=1e-4)
+    assert (out[..., :lo] == 7).all() and (out[..., hi:] == 7).all()
+    a = norm.group_norm_backward(dys.contiguous(), xs.contiguous(), st0, 2, g, b, act="gelu", dropout=drop)
+    dxo = torch.full_like(x, 7.0)
+    d = norm.group_norm_backward(dys, xs, st0, 2, g, b, act="gelu", dropout=drop, dx=dxo[..., lo:hi])
+    assert torch.allclose(a[0].double(), d[0].double(), rtol=tol, atol=1e-3) and torch.allclose(a[1], d[1], rtol=1e-4, atol=1e-4) and torch.allclose(a[2], d[2], rtol=1e-4, atol=1e-4)
+    assert (dxo[..., :lo] == 7).all() and (dxo[..., hi:] == 7).all()
+
+
+def test_in_place(env):
+    torch, norm = env
+    x, dy, gamma, beta = _inputs(torch, 3, 33, 31, 32, "bf16", 11)
+    y, st = norm.group_norm(x, 4, gamma, beta, act="silu")
+    dx, _, _ = norm.group_norm_backward(dy, x, st, 4, gamma, beta, act="silu")
+    xi, di = x.clone(), dy.clone()
+    yi, sti = norm.group_norm(xi, 4, gamma, beta, act="silu", out=xi)
+    assert yi.data_ptr() == xi.data_ptr() and torch.equal(yi, y) and torch.equal(sti, st)
+    norm.group_norm_backward(di, x, st, 4, gamma, beta, act="silu", dx=di)
+    assert torch.equal(di, dx)
+
+
+@pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_what_is_not_finite_stays_in_its_group(env, act, bad):
+    torch, norm = env
+    x, dy, gamma, beta = _inputs(torch, 2, 20, 20, 16, "f32", 12)
+    y0, st0 = norm.group_norm(x, 4, gamma, beta, act=act)
+    d0 = norm.group_norm_backward(dy, x, st0, 4, gamma, beta, act=act)
+    x2 = x.clone()
+    x2[1, 3, 4, 5] = bad                                    # image 1, group 1
+    y, st = norm.group_norm(x2, 4, gamma, beta, act=act)
+    assert torch.isnan(y[1, :, :, 4:8]).all() and torch.isnan(st[1, 1, 1])
+    keep = torch.ones_like(y, dtype=torch.bool)
+    keep[1, :, :, 4:8] = False
+    assert torch.equal(y[keep], y0[keep])
+    d = norm.group_norm_backward(dy, x2, st, 4, gamma, beta, act=act)
+    assert torch.equal(d[0][keep], d0[0][keep]) and torch.isnan(d[1][4:8]).all()
+    others = torch.tensor([k for k in range(16) if not 4 <= k < 8], device="cuda:0")
+    assert torch.equal(d[1][others], d0[1][others])
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("count", [1, 7, 8, 9, 64, 1000, 4095, 73728, 1000003])
+@pytest.mark.parametrize("p", [0.0, 1e-3, 0.1, 0.5, 0.999, 1.0])
+def test_dropout_vs_oracle(env, t, count, p):
+    torch, norm = env
+    r = np.random.default_rng(count)
+    x, res = (_to(torch, r.standard_normal(count), t) for _ in range(2))
+    seed, offset = (1 << 63) + 12345, 999999999999
+    fac = no.drop_factor((count,), p, seed, offset)
+    drop = norm.Dropout(p, seed, offset)
+    got = _np(norm.dropout(x, drop))
+    want = _np(x) * fac
+    assert np.array_equal(got == 0, (want == 0))
+    _within(got, want, (HALF[t] + 2 * E) * np.abs(want) + TINY[t], "dropout")
+    want = want + _np(res)
+    got = _np(norm.dropout(x, drop, residual=res))
+    _within(got, want, HALF[t] * np.abs(want) + 3 * E * (np.abs(want) + np.abs(_np(x) * fac)) + TINY[t], "with residual")
+    # the gradient has the same mask
+    assert torch.equal(norm.dropout_backward(x, drop), norm.dropout(x, drop))
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+def test_dropout_in_place_and_unaligned(env, t):
+    torch, norm = env
+    buf, rbuf = (torch.randn(5003, device="cuda:0").to(_type(torch, t)) for _ in range(2))
+    drop = norm.Dropout(0.4, 3, 4)
+    for off in (0, 1, 3, 8):
+        x, res = buf[off:off + 4999 - off], rbuf[off:off + 4999 - off]
+        want = norm.dropout(x.clone(), drop, residual=res.clone())
+        assert torch.equal(norm.dropout(x, drop, residual=res), want)
+        wide = torch.full((5003,), 7.0, device="cuda:0", dtype=x.dtype)
+        v = wide[off:off + 4999 - off]
+        v.copy_(x)
+        norm.dropout(v, drop, residual=res, out=v)
+        assert torch.equal(v, want) and (wide[:off] == 7).all() and (wide[4999:] == 7).all()
+
+
+def test_dropped_values_are_zero_whatever_they_were(env):
+    torch, norm = env
+    x = torch.full((4096,), float("nan"), device="cuda:0")
+    x[::2] = float("inf")
+    drop = norm.Dropout(0.5, 21, 22)
+    kept = torch.from_numpy(no.drop_factor((4096,), 0.5, 21, 22) > 0).cuda()
+    y = norm.dropout(x, drop, residual=torch.ones_like(x))
+    assert (y[~kept] == 1).all() and not torch.isfinite(y[kept]).any()
+    # ... and in the fused form: what the mask drops of the gradient is not read
+    xx, dy, gamma, beta = _inputs(torch, 1, 16, 16, 16, "f32", 1)
+    _, st = norm.group_norm(xx, 2, gamma, beta, act="silu", dropout=drop)
+    d0 = norm.group_norm_backward(dy, xx, st, 2, gamma, beta, act="silu", dropout=drop)
+    dy2 = torch.where(kept.view(dy.shape), dy, torch.full_like(dy, float("nan")))
+    d1 = norm.group_norm_backward(dy2, xx, st, 2, gamma, beta, act="silu", dropout=drop)
+    assert all(torch.equal(a, b) for a, b in zip(d0, d1))
+
+
+def test_fused_dropout_is_the_dropout_operator(env):
+    torch, norm = env
+    for c, t in ((32, "f32"), (36, "f16"), (29, "bf16"), (6, "f32")):
+        x, dy, gamma, beta = _inputs(torch, 2, 9, 10, c, t, 31)
+        drop = norm.Dropout(0.2, 8, 9)
+        y, _ = norm.group_norm(x, 1, gamma, beta, act="none", dropout=drop)
+        mask = norm.dropout(torch.ones_like(x), drop)
+        assert torch.equal(y == 0, mask == 0), c
+
+
+def test_same_bits_every_time_and_on_streams(env):
+    torch, norm = env
+    x, dy, gamma, beta = _inputs(torch, 4, 61, 47, 64, "f32", 17)
+    drop = norm.Dropout(0.1, 8, 9)
+
+    def once():
+        y, st = norm.group_norm(x, 8, gamma, beta, act="silu", dropout=drop)
+        return (y, st) + norm.group_norm_backward(dy, x, st, 8, gamma, beta, act="silu", dropout=drop)
+
+    want = once()
+    torch.cuda.synchronize()
+    side = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for _ in range(3):
+        for s in side:                                      # two at once, each with a workspace of its own
+            with torch.cuda.stream(s):
+                got.append(once())
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
+
+
+def test_captured_and_replayed(env):
+    """A block's forward and backward in one graph: with the counter advanced before each replay, every replay equals the eager calls with
+    that number; eager work of the same inputs runs in between."""
+    torch, norm = env
+    x, dy, gamma, beta = _inputs(torch, 2, 30, 26, 64, "bf16", 23)
+    counter = torch.zeros(1, dtype=torch.int64, device="cuda:0")
+
+    def once(drop, drop2):
+        y, st = norm.group_norm(x, 8, gamma, beta, act="silu", dropout=drop)
+        z = norm.dropout(y, drop2, residual=x)
+        g = norm.dropout_backward(dy, drop2)
+        return (y, st, z, g) + norm.group_norm_backward(g, x, st, 8, gamma, beta, act="silu", dropout=drop)
+
+    pair = norm.Dropout(0.1, 5, 100, counter), norm.Dropout(0.3, 5, 1 << 33, counter)
+    once(*pair)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = once(*pair)
+    seen = []
+    for k in (0, 1, 2, 7, 1 << 35):
+        counter.fill_(k)
+        graph.replay()
+        want = once(norm.Dropout(0.1, 5, 100 + k), norm.Dropout(0.3, 5, (1 << 33) + k))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), k
+        seen.append(out[0].clone())
+    assert not torch.equal(seen[0], seen[1])
+
+
+def test_gradients_against_differences(env):
+    """The loss sum(y * r) along random directions.  Central differences with h = 2^-6: the third derivative of the loss along a unit-size
+    direction is below 50 here (h^2 / 6 * 50 = 2e-3); outputs are off by at most 2e-6 each, 4000 of them at random: 2e-6 * 63 / h = 8e-3."""
+    torch, norm = env
+    n, h, w, c = 2, 10, 10, 20
+    x, r, gamma, beta = _inputs(torch, n, h, w, c, "f32", 41)
+    drop = norm.Dropout(0.25, 1, 2)
+    _, st = norm.group_norm(x, 4, gamma, beta, act="gelu", dropout=drop)
+    grads = norm.group_norm_backward(r, x, st, 4, gamma, beta, act="gelu", dropout=drop)
+    loss = lambda *a: float((norm.group_norm(a[0], 4, a[1], a[2], act="gelu", dropout=drop)[0].double() * r.double()).sum())  # noqa: E731
+    gen = torch.Generator(device="cuda:0").manual_seed(5)
+    leaves, step = [x, gamma, beta], 2.0 ** -6
+    for k in range(3):
+        v = torch.randn(leaves[k].shape, device="cuda:0", generator=gen)
+        v /= v.norm()
+        hi, lo = ([q + s * step * v if j == k else q for j, q in enumerate(leaves)] for s in (1, -1))
+        num = (loss(*hi) - loss(*lo)) / (2 * step)
+        assert abs(num - float((grads[k].double() * v.double()).sum())) < 1e-2, k
+
+
+def test_offsets_past_32_bits(env):
+    """More than 2^32 elements: the last ones' mask and normalisation are theirs (a 32-bit index would take the first ones')."""
+    torch, norm = env
+    count = (1 << 32) + (1 << 20) + 24
+    x = torch.ones(count, dtype=torch.bfloat16, device="cuda:0")
+    norm.dropout(x, norm.Dropout(0.5, 77, 78), out=x)
+    for first in (0, (1 << 31) - 512, (1 << 32) - 512, count - 1024):
+        want = no.drop_factor((1024,), 0.5, 77, 78, first)
+        assert np.array_equal(_np(x[first:first + 1024]), want), first
+    del x
+    n, h, w, c = 3, 4731, 4733, 64                          # 4.3e9 elements, half a type's step of bf16 around 1
+    x = torch.empty(n, h, w, c, dtype=torch.bfloat16, device="cuda:0")
+    gen = torch.Generator(device="cuda:0").manual_seed(3)
+    block = torch.randn(1, 1, w, c, device="cuda:0", generator=gen)
+    for i in range(n):
+        x[i] = (block * (i + 1) + i).to(torch.bfloat16)     # every row of an image alike: its statistics are the row's
+    assert x.numel() > 1 << 32
+    drop = norm.Dropout(0.25, 5, 6)
+    y, st = norm.group_norm(x, 4, act="none", dropout=drop, out=x)
+    for i in range(n):
+        row = (block * (i + 1) + i).to(torch.bfloat16).double().cpu().numpy()
+        mean, rstd = no.stats(row, 4, 1e-5)
+        # sums of 1.4e9 values: threads' chains of 700 batches, K E -> 1e-4 relative at the most
+        assert np.abs(_np(st[0, i]) - mean[0]).max() < 1e-4 * (i + 1) and np.abs(_np(st[1, i]) / rstd[0] - 1).max() < 1e-4
+        first = (i * h * w + (h - 1) * w) * c               # the image's last row
+        want = (row - no.per_channel(mean, c)) * no.per_channel(rstd, c) * no.drop_factor(row.shape, 0.25, 5, 6, first)
+        got = _np(y[i, h - 1])
+        assert np.abs(got - want[0, 0]).max() < 2.0 ** -8 * 6 + 1e-3, i
+        assert np.array_equal(got == 0, want[0, 0] == 0)
