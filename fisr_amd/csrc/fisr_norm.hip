@@ -2,6 +2,7 @@
 // its own: its device code is compiled without packed float32 instructions (fisr_amd/lib.py), which the Winograd kernels of
 // fisr_api.hip write by hand.
 #include <cmath>
+#include <cstdlib>
 
 #include "../../include/fisr.h"
 #include "host_util.h"
@@ -17,56 +18,171 @@ using namespace fisr;
 
 namespace {
 
-// Chunks of one image: about 2048 workgroups for the whole batch (8 a CU), of at least 8192 elements each (32 a thread).  Not a
-// function of the vector width: the workspace's size is asked for without the tensors.
-void norm_chunks(NormArgs& a) {
-  const int want = std::max(1, 2048 / a.n);
-  a.ppc = std::max((a.p + want - 1) / want, (8191 + a.c) / a.c);
-  a.chunks = (a.p + a.ppc - 1) / a.ppc;
+#ifdef FISR_DIAG
+int env_int(const char* name, int def) { const char* e = getenv(name); return e ? atoi(e) : def; }
+#else
+constexpr int env_int(const char*, int def) { return def; }
+#endif
+
+// Chunks of an image's pixels for about `groups` workgroups in all, of at least 8192 elements each (32 a thread).
+void chunks_for(const NormArgs& a, int workgroups, int& chunks, int& ppc) {
+  const int want = std::max(1, workgroups / a.n);
+  ppc = std::max((a.p + want - 1) / want, (8191 + a.c) / a.c);
+  chunks = (a.p + ppc - 1) / ppc;
 }
-void norm_threads(NormArgs& a, int v, dim3& grid) {
-  const int cv = (a.c + v - 1) / v, ny = (cv + 255) / 256;
-  a.cb = (cv + ny - 1) / ny;
-  a.rows = 256 / a.cb;
-  grid = dim3(a.n * a.chunks, ny);
+constexpr int MOST_CHUNK_GROUPS = 2048;                          // of a batch, by chunks_for: what the workspace is made for
+
+// Workspace: `part` of n * chunks * c float2, and for the backward pass s12 of n * groups * chunks and ab of n * c.  Not a function of the
+// vector width or the form that runs: its size is asked for without the tensors.
+struct WsLayout { size_t part, s12, ab; };
+WsLayout ws_layout(const NormArgs& a, bool backward) {
+  int chunks, ppc;
+  chunks_for(a, MOST_CHUNK_GROUPS, chunks, ppc);
+  WsLayout w{(size_t)a.n * chunks * a.c, 0, 0};
+  if (backward) { w.s12 = (size_t)a.n * a.groups * chunks; w.ab = (size_t)a.n * a.c; }
+  return w;
 }
 size_t norm_ws_bytes(const NormArgs& a, bool backward) {
-  size_t f2 = (size_t)a.n * a.chunks * a.c;
-  if (backward) f2 += (size_t)a.n * a.c + (size_t)a.n * a.groups;
-  return f2 * sizeof(float2);
+  const WsLayout w = ws_layout(a, backward);
+  return (w.part + w.s12 + w.ab) * sizeof(float2);
 }
 
-// One pixel of a launch's workgroups: vectors of eight channels where all tensors allow 16-byte accesses, else four or two, else one.
+// Vectors of 16 bytes where all tensors allow such accesses, else of 8 and so on down to one channel.
 template <typename T> int norm_vec(const NormArgs& a) {
   const uintptr_t ptrs = (uintptr_t)a.x | (uintptr_t)a.dy | (uintptr_t)a.y;
   const size_t cs = a.xcs | a.ycs | a.dycs;
-  for (int v = 8; v > 1; v >>= 1) {
-    const size_t bytes = std::min<size_t>(v * sizeof(T), 16);
-    if (a.c % v == 0 && ptrs % bytes == 0 && cs * sizeof(T) % bytes == 0) return v;
-  }
+  for (int v = 16 / sizeof(T); v > 1; v >>= 1)
+    if (a.c % v == 0 && ptrs % (v * sizeof(T)) == 0 && cs * sizeof(T) % (v * sizeof(T)) == 0) return v;
   return 1;
 }
-
-template <typename T, int V> void launch_fwd(NormArgs a, hipStream_t st) {
-  dim3 grid;
-  norm_threads(a, V, grid);
-  hipLaunchKernelGGL((norm_stats_kernel<T, V>), grid, dim3(256), 0, st, a);
-  hipLaunchKernelGGL(norm_stats_join_kernel, dim3(a.n * a.groups), dim3(256), 0, st, a);
-  hipLaunchKernelGGL((norm_apply_kernel<T, V>), grid, dim3(256), 0, st, a);
+uint32_t magic(int y) { return y == 1 ? 0 : (uint32_t)(((1ull << 32) + y - 1) / y); }
+// A workgroup's columns, rows and what team_sums goes by.
+void set_team(NormArgs& a, int v, int threads, int span) {
+  a.span = span; a.cb = span / v; a.rows = threads / a.cb;
+  a.slots = a.d % v == 0 ? 1 : v % a.d == 0 ? v / a.d : v;
+  a.per_group = a.d * a.slots / v;
+  a.by_cb = magic(a.cb); a.by_rows = magic(a.rows); a.by_per_group = magic(a.per_group);
+  const int groups = span / a.d;
+  for (a.jl = 6; a.jl > 0 && groups > threads >> a.jl;) --a.jl;
 }
-template <typename T, int V> void launch_bwd(NormArgs a, hipStream_t st) {
-  dim3 grid;
-  norm_threads(a, V, grid);
+// lcm(d, v): the least channels that are whole groups and whole vectors
+int span_unit(const NormArgs& a, int v) {
+  int unit = a.d;
+  while (unit % v) unit += a.d;
+  return unit;
+}
+
+// One launch, a span of channels of a whole image in a workgroup's registers: which variant holds it (-1: none).
+struct TeamVariant { int threads, r; };
+constexpr TeamVariant TEAM[] = {{256, 1}, {256, 2}, {256, 4}, {256, 9}, {512, 9}};
+int team_variant(NormArgs& a, int v, int elem_bytes) {
+  const int unit = span_unit(a, v), most = a.c / unit;
+  int best = -1, best_span = 0;
+  for (int k = 1; k <= most; ++k) {
+    if (most % k) continue;
+    const int span = k * unit, cols = span / v;
+    if (cols > 256) break;
+    // wider spans up to whole 128-byte lines, then as long as there are two workgroups a CU (256 CUs)
+    if (best >= 0 && best_span * elem_bytes >= env_int("NORM_SPAN", 64) && (long long)a.n * (a.c / span) < env_int("NORM_TWG", 512)) break;
+    int fit = -1;
+    for (int i = 0; i < (int)(sizeof(TEAM) / sizeof(TEAM[0])) && fit < 0; ++i) {
+      const int rows = TEAM[i].threads / cols;
+      if ((a.p + rows - 1) / rows <= TEAM[i].r) fit = i;
+    }
+    if (fit < 0) break;
+    best = fit; best_span = span;
+  }
+  if (best >= 0) set_team(a, v, TEAM[best].threads, best_span);
+  return best;
+}
+bool team_wins(const NormArgs& a, int elem_bytes, bool backward) {
+  const size_t bytes = (size_t)a.n * a.p * a.c * elem_bytes;
+  return bytes <= (size_t)env_int(backward ? "NORM_TEAMB_KB" : "NORM_TEAM_KB", 32768) << 10;
+}
+template <typename T, int V> bool launch_team(NormArgs a, bool backward, hipStream_t st) {
+  const int variant = team_variant(a, V, sizeof(T));
+  if (variant < 0) return false;
+  const dim3 grid(a.n * (a.c / a.span));
+#define NORM_TEAM(I)                                                                                                                         \
+  case I:                                                                                                                                    \
+    if (backward) hipLaunchKernelGGL((norm_team_grad_kernel<T, V, TEAM[I].r, TEAM[I].threads>), grid, dim3(TEAM[I].threads), 0, st, a);       \
+    else hipLaunchKernelGGL((norm_team_kernel<T, V, TEAM[I].r, TEAM[I].threads>), grid, dim3(TEAM[I].threads), 0, st, a);                     \
+    break;
+  switch (variant) { NORM_TEAM(0) NORM_TEAM(1) NORM_TEAM(2) NORM_TEAM(3) NORM_TEAM(4) }
+#undef NORM_TEAM
+  if (backward && (a.dgamma || a.dbeta)) hipLaunchKernelGGL(norm_params_kernel, dim3((a.c + 15) / 16), dim3(256), 0, st, a, a.ab, a.n);
+  return true;
+}
+
+// Two launches over chunks of pixels: grids and the channels of a workgroup (all, or the most whole groups that it has threads for).
+bool two_tiling(NormArgs& a, int v, int elem_bytes, bool backward) {
+  const int unit = span_unit(a, v), most = a.c / unit;
+  int k = most;
+  while (k > 0 && (most % k || k * unit / v > 256)) --k;
+  if (k == 0) return false;
+  set_team(a, v, 256, k * unit);
+  // first launch: long-lived workgroups (their numbers have to be joined); second: some 48 KB each, four a CU at least
+  const size_t bytes = (size_t)a.n * a.p * a.c * elem_bytes * (backward ? 2 : 1);
+  chunks_for(a, env_int("NORM_SWG", bytes > (size_t)128 << 20 ? 1024 : 512), a.chunks, a.ppc);
+  chunks_for(a, env_int("NORM_AWG", (int)std::min<size_t>(std::max<size_t>(bytes / 49152, 1024), 16384)), a.achunks, a.appc);
+  return true;
+}
+template <typename T, int V, bool NT> void launch_two_nt(NormArgs a, bool backward, hipStream_t st) {
+  constexpr int TH = 256;
+  const int ny = a.c / a.span;
+  const dim3 g1(a.n * a.chunks, ny);
+  if (backward) {
+    const int pblocks = a.dgamma || a.dbeta ? (a.c + 15) / 16 : 0;
+    hipLaunchKernelGGL((norm_chunk_sums_kernel<T, V, TH, NT>), g1, dim3(TH), 0, st, a);
+    hipLaunchKernelGGL((norm_chunk_grad_kernel<T, V, TH, NT>), dim3(pblocks + a.n * a.achunks, ny), dim3(TH), 0, st, a, pblocks);
+    return;
+  }
+  const int join = a.chunks * (a.span / a.d) <= env_int("NORM_JOIN", 2048);
+  hipLaunchKernelGGL((norm_chunk_stats_kernel<T, V, TH, NT>), g1, dim3(TH), 0, st, a);
+  if (!join) {
+    NormArgs b = a;
+    b.jl = 6;
+    hipLaunchKernelGGL(norm_join_kernel, dim3(a.n * a.groups), dim3(64), 0, st, b);
+  }
+  hipLaunchKernelGGL((norm_chunk_apply_kernel<T, V, TH, NT>), dim3(a.n * a.achunks, ny), dim3(TH), 0, st, a, join);
+}
+template <typename T, int V> bool launch_two(NormArgs a, bool backward, hipStream_t st) {
+  if (!two_tiling(a, V, sizeof(T), backward)) return false;
+  const size_t bytes = (size_t)a.n * a.p * a.c * sizeof(T) * (backward ? 2 : 1);
+  if (bytes > (size_t)env_int("NORM_NT_MB", 128) << 20) launch_two_nt<T, V, true>(a, backward, st);
+  else launch_two_nt<T, V, false>(a, backward, st);
+  return true;
+}
+
+// Any shape.
+template <typename T, int V> void launch_any(NormArgs a, bool backward, hipStream_t st) {
+  chunks_for(a, MOST_CHUNK_GROUPS, a.chunks, a.ppc);
+  const int cv = (a.c + V - 1) / V, ny = (cv + 255) / 256;
+  a.cb = (cv + ny - 1) / ny;
+  a.rows = 256 / a.cb;
+  const dim3 grid(a.n * a.chunks, ny);
+  if (!backward) {
+    hipLaunchKernelGGL((norm_stats_kernel<T, V>), grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL(norm_stats_join_kernel, dim3(a.n * a.groups), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((norm_apply_kernel<T, V>), grid, dim3(256), 0, st, a);
+    return;
+  }
   hipLaunchKernelGGL((norm_bwd_sums_kernel<T, V>), grid, dim3(256), 0, st, a);
   hipLaunchKernelGGL(norm_bwd_join_kernel, dim3(a.n * a.groups), dim3(256), 0, st, a);
   hipLaunchKernelGGL((norm_bwd_apply_kernel<T, V>), grid, dim3(256), 0, st, a);
-  if (a.dgamma || a.dbeta) hipLaunchKernelGGL(norm_bwd_params_kernel, dim3((a.c + 63) / 64), dim3(256), 0, st, a);
+  if (a.dgamma || a.dbeta) hipLaunchKernelGGL(norm_params_kernel, dim3((a.c + 15) / 16), dim3(256), 0, st, a, a.ab, a.n);
+}
+template <typename T, int V> void launch_v(const NormArgs& a, bool backward, hipStream_t st) {
+  if (team_wins(a, sizeof(T), backward) && launch_team<T, V>(a, backward, st)) return;
+  if (!launch_two<T, V>(a, backward, st)) launch_any<T, V>(a, backward, st);
 }
 template <typename T> void launch(const NormArgs& a, bool backward, hipStream_t st) {
-  const int v = norm_vec<T>(a);
-#define NORM_V(V) if (v == V) { if (backward) launch_bwd<T, V>(a, st); else launch_fwd<T, V>(a, st); return; }
-  NORM_V(8) NORM_V(4) NORM_V(2) NORM_V(1)
-#undef NORM_V
+  switch (norm_vec<T>(a)) {
+    case 8: if constexpr (sizeof(T) == 2) launch_v<T, 8>(a, backward, st); break;
+    case 4: launch_v<T, 4>(a, backward, st); break;
+    case 2: launch_v<T, 2>(a, backward, st); break;
+    default: launch_v<T, 1>(a, backward, st);
+  }
 }
 
 // The shape's limits keep every pixel index in 31 bits and every grid in HIP's (elements are counted in 64 bits).
@@ -100,14 +216,14 @@ int norm_call(const char* who, NormArgs& a, bool backward, int n, int h, int w, 
     return bad("a pointer is not aligned to its element");
   if (act < FISR_ACT_NONE || act > FISR_ACT_GELU) return bad("unknown activation");
   if (const char* e = drop_error(drop, a.drop)) return bad(e);
-  a.n = n; a.p = h * w; a.c = c; a.groups = groups; a.d = c / groups; a.act = act;
+  a.n = n; a.p = h * w; a.c = c; a.groups = groups; a.d = c / groups; a.by_d = magic(a.d); a.act = act;
   a.mean = mean_rstd; a.rstd = mean_rstd + (size_t)n * groups;
-  norm_chunks(a);
   if (!ws || (uintptr_t)ws % 16) return bad("the workspace is null or not aligned to 16 bytes");
   if (ws_bytes < norm_ws_bytes(a, backward)) return set_error(FISR_ENOMEM, std::string(who) + ": workspace too small");
+  const WsLayout lay = ws_layout(a, backward);
   a.part = (float2*)ws;
-  a.ab = a.part + (size_t)a.n * a.chunks * a.c;
-  a.s12 = a.ab + (size_t)a.n * a.c;
+  a.s12 = a.part + lay.part;
+  a.ab = a.s12 + lay.s12;
   DeviceGuard guard(device_of(a.y));
   NORM_HIP_OK(guard.err);
   const hipStream_t st = (hipStream_t)stream;
@@ -133,7 +249,6 @@ size_t fisr_train_groupnorm_workspace_bytes(int n, int h, int w, int c, int grou
   if (norm_shape_error(n, h, w, c, groups)) return 0;
   NormArgs a{};
   a.n = n; a.p = h * w; a.c = c; a.groups = groups;
-  norm_chunks(a);
   return norm_ws_bytes(a, backward != 0);
 }
 
