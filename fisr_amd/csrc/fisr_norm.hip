@@ -18,6 +18,7 @@ using namespace fisr;
 
 namespace {
 
+
 #ifdef FISR_DIAG
 int env_int(const char* name, int def) { const char* e = getenv(name); return e ? atoi(e) : def; }
 #else
@@ -51,7 +52,7 @@ size_t norm_ws_bytes(const NormArgs& a, bool backward) {
 template <typename T> int norm_vec(const NormArgs& a) {
   const uintptr_t ptrs = (uintptr_t)a.x | (uintptr_t)a.dy | (uintptr_t)a.y;
   const size_t cs = a.xcs | a.ycs | a.dycs;
-  for (int v = 16 / sizeof(T); v > 1; v >>= 1)
+  for (int v = std::min<int>(16 / sizeof(T), env_int(a.dy ? "NORM_VB" : "NORM_VF", 8)); v > 1; v >>= 1)
     if (a.c % v == 0 && ptrs % (v * sizeof(T)) == 0 && cs * sizeof(T) % (v * sizeof(T)) == 0) return v;
   return 1;
 }
@@ -72,18 +73,20 @@ int span_unit(const NormArgs& a, int v) {
   return unit;
 }
 
-// One launch, a span of channels of a whole image in a workgroup's registers: which variant holds it (-1: none).
+// One launch, a span of channels of a whole image in a workgroup's registers: which variant holds it (-1: none does, or it would be slower).
 struct TeamVariant { int threads, r; };
 constexpr TeamVariant TEAM[] = {{256, 1}, {256, 2}, {256, 4}, {256, 9}, {512, 9}};
-int team_variant(NormArgs& a, int v, int elem_bytes) {
+int team_variant(NormArgs& a, int v, int elem_bytes, bool backward) {
+  const size_t elems = (size_t)a.n * a.p * a.c;
+  if (elems > (size_t)env_int("NORM_TEAM_K", 16384) << 10) return -1;
   const int unit = span_unit(a, v), most = a.c / unit;
+  const int line = elems * elem_bytes > (size_t)4 << 20 ? 64 : 16;  // least bytes of a span: narrow ones read a cache line many times over
   int best = -1, best_span = 0;
   for (int k = 1; k <= most; ++k) {
     if (most % k) continue;
     const int span = k * unit, cols = span / v;
     if (cols > 256) break;
-    // wider spans up to whole 128-byte lines, then as long as there are two workgroups a CU (256 CUs)
-    if (best >= 0 && best_span * elem_bytes >= env_int("NORM_SPAN", 64) && (long long)a.n * (a.c / span) < env_int("NORM_TWG", 512)) break;
+    if (best >= 0 && best_span * elem_bytes >= line && (best_span * elem_bytes >= 128 || (long long)a.n * (a.c / span) < 512)) break;
     int fit = -1;
     for (int i = 0; i < (int)(sizeof(TEAM) / sizeof(TEAM[0])) && fit < 0; ++i) {
       const int rows = TEAM[i].threads / cols;
@@ -92,26 +95,22 @@ int team_variant(NormArgs& a, int v, int elem_bytes) {
     if (fit < 0) break;
     best = fit; best_span = span;
   }
+  // few workgroups of many vectors a thread: the two launches' finer chunks are faster (one image of 48 x 48 x 128 bf16, 8 workgroups:
+  // 12.8 us against 12.3, backward 20.1 against 14.9; with 32 workgroups of at most 4 vectors 8.3 against 11.5, backward 10.6 against 14.4)
+  if (best >= 0 && TEAM[best].r > 4 && (backward || TEAM[best].threads > 256) && (long long)a.n * (a.c / best_span) < 64) best = -1;
   if (best >= 0) set_team(a, v, TEAM[best].threads, best_span);
   return best;
 }
-bool team_wins(const NormArgs& a, int elem_bytes, bool backward) {
-  const size_t bytes = (size_t)a.n * a.p * a.c * elem_bytes;
-  return bytes <= (size_t)env_int(backward ? "NORM_TEAMB_KB" : "NORM_TEAM_KB", 32768) << 10;
-}
-template <typename T, int V> bool launch_team(NormArgs a, bool backward, hipStream_t st) {
-  const int variant = team_variant(a, V, sizeof(T));
-  if (variant < 0) return false;
+template <typename T, int V> void launch_team(const NormArgs& a, bool backward, hipStream_t st) {
   const dim3 grid(a.n * (a.c / a.span));
 #define NORM_TEAM(I)                                                                                                                         \
   case I:                                                                                                                                    \
     if (backward) hipLaunchKernelGGL((norm_team_grad_kernel<T, V, TEAM[I].r, TEAM[I].threads>), grid, dim3(TEAM[I].threads), 0, st, a);       \
     else hipLaunchKernelGGL((norm_team_kernel<T, V, TEAM[I].r, TEAM[I].threads>), grid, dim3(TEAM[I].threads), 0, st, a);                     \
     break;
-  switch (variant) { NORM_TEAM(0) NORM_TEAM(1) NORM_TEAM(2) NORM_TEAM(3) NORM_TEAM(4) }
+  switch (a.team) { NORM_TEAM(0) NORM_TEAM(1) NORM_TEAM(2) NORM_TEAM(3) NORM_TEAM(4) }
 #undef NORM_TEAM
   if (backward && (a.dgamma || a.dbeta)) hipLaunchKernelGGL(norm_params_kernel, dim3((a.c + 15) / 16), dim3(256), 0, st, a, a.ab, a.n);
-  return true;
 }
 
 // Two launches over chunks of pixels: grids and the channels of a workgroup (all, or the most whole groups that it has threads for).
@@ -173,7 +172,7 @@ template <typename T, int V> void launch_any(NormArgs a, bool backward, hipStrea
   if (a.dgamma || a.dbeta) hipLaunchKernelGGL(norm_params_kernel, dim3((a.c + 15) / 16), dim3(256), 0, st, a, a.ab, a.n);
 }
 template <typename T, int V> void launch_v(const NormArgs& a, bool backward, hipStream_t st) {
-  if (team_wins(a, sizeof(T), backward) && launch_team<T, V>(a, backward, st)) return;
+  if (a.team >= 0) return launch_team<T, V>(a, backward, st);
   if (!launch_two<T, V>(a, backward, st)) launch_any<T, V>(a, backward, st);
 }
 template <typename T> void launch(const NormArgs& a, bool backward, hipStream_t st) {
@@ -218,8 +217,9 @@ int norm_call(const char* who, NormArgs& a, bool backward, int n, int h, int w, 
   if (const char* e = drop_error(drop, a.drop)) return bad(e);
   a.n = n; a.p = h * w; a.c = c; a.groups = groups; a.d = c / groups; a.by_d = magic(a.d); a.act = act;
   a.mean = mean_rstd; a.rstd = mean_rstd + (size_t)n * groups;
-  if (!ws || (uintptr_t)ws % 16) return bad("the workspace is null or not aligned to 16 bytes");
-  if (ws_bytes < norm_ws_bytes(a, backward)) return set_error(FISR_ENOMEM, std::string(who) + ": workspace too small");
+  if ((uintptr_t)ws % 16) return bad("the workspace is not aligned to 16 bytes");
+  a.team = team_variant(a, es == 4 ? norm_vec<float>(a) : norm_vec<f16_t>(a), (int)es, backward);
+  if ((backward || a.team < 0) && (!ws || ws_bytes < norm_ws_bytes(a, backward))) return set_error(FISR_ENOMEM, std::string(who) + ": workspace too small");
   const WsLayout lay = ws_layout(a, backward);
   a.part = (float2*)ws;
   a.s12 = a.part + lay.part;

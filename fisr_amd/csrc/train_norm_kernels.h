@@ -200,7 +200,7 @@ struct NormArgs {
   int achunks, appc;                                   // ... in the second of two launches
   int slots, per_group, jl;                            // see team_sums
   uint32_t by_d, by_cb, by_rows, by_per_group;               // for div_by
-  float eps; int act, accumulate;
+  float eps; int act, accumulate, team;                // team: the host's variant of the one-launch form
   DropArgs drop;
 };
 // x / y for x < 2^16 and y <= 2^16 by the host's ceil(2^32 / y) (0 for y = 1): a division by a number of the launch is some 20 instructions
@@ -712,7 +712,7 @@ template <typename T, int V> struct GradPixels {
 
 // First launch: part[image][chunk][channel] = (A, B) of a chunk, and behind it s12[image][group][chunk] = (sum of gamma A, of gamma B) / (P D).
 template <typename T, int V, int TH, bool NT> __global__ __launch_bounds__(TH) void norm_chunk_sums_kernel(const NormArgs a) {
-  constexpr int U = 2;
+  constexpr int U = sizeof(T) * V == 8 ? 4 : 2;
   __shared__ float2 sum[TH * V];
   __shared__ float2 tot[TH * V];
   int chunk, p0, p1;
@@ -778,7 +778,7 @@ __global__ __launch_bounds__(256) void norm_params_kernel(const NormArgs a, cons
 // Second launch: dx.  Its first `pblocks` workgroups sum the parameters' gradients instead.
 template <typename T, int V, int TH, bool NT> __global__ __launch_bounds__(TH) void norm_chunk_grad_kernel(const NormArgs a, int pblocks) {
   static_assert(TH == 256, "param_grads");
-  constexpr int U = 2;
+  constexpr int U = sizeof(T) * V == 8 ? 4 : 2;
   __shared__ float2 tot[TH * V];
   if ((int)blockIdx.x < pblocks) {
     if (blockIdx.y == 0) param_grads(a, a.part, a.n * a.chunks, blockIdx.x);

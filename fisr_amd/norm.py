@@ -25,6 +25,7 @@ ACTIVATIONS = {"none": _lib.ACT_NONE, "relu": _lib.ACT_RELU, "silu": _lib.ACT_SI
 _TYPES = {torch.float32: _lib.TYPE_F32, torch.float16: _lib.TYPE_F16, torch.bfloat16: _lib.TYPE_BF16}
 _M64 = (1 << 64) - 1
 _INT = (1 << 31) - 1
+_ENOMEM = -5                                           # FISR_ENOMEM: the workspace is too small
 
 
 class Dropout:
@@ -44,9 +45,19 @@ class Dropout:
         self.desc = _lib.DropoutDesc(p, int(seed) & _M64, int(offset) & _M64, counter.data_ptr() if counter is not None else None)
 
 
-def _check(rc):
-    if rc < 0:
-        raise _lib.FisrError(f"libfisr_hip error {rc}: {_lib.lib().fisr_last_error(None).decode('utf-8', 'replace')}")
+class _Entries:
+    """The library's entry points, found on first use."""
+
+    def __getattr__(self, name):
+        if name not in ("gn", "gn_bwd", "drop", "ws_bytes"):
+            raise AttributeError(name)
+        L = _lib.lib()
+        self.gn, self.gn_bwd, self.drop, self.ws_bytes = (L.fisr_train_groupnorm, L.fisr_train_groupnorm_bwd, L.fisr_train_dropout,
+                                                          L.fisr_train_groupnorm_workspace_bytes)
+        return self.__dict__[name]
+
+
+_fn = _Entries()
 
 
 def _pixel_stride(t, what):
@@ -63,28 +74,36 @@ def _pixel_stride(t, what):
     return cs
 
 
-def _images(x, what, groups):
-    if x.dim() != 4:
-        raise ValueError(f"{what}: [N, H, W, C] is wanted, got {tuple(x.shape)}")
-    if max(x.shape) > _INT or not -1 <= groups <= _INT:
-        raise ValueError(f"{what}: {tuple(x.shape)} in {groups} groups: a size is too large")
-    if x.dtype not in _TYPES:
-        raise ValueError(f"{what}: float32, float16 or bfloat16 is wanted, got {x.dtype}")
+def _type(x):
+    """The library's number of x's type, and the index of its device."""
+    code = _TYPES.get(x.dtype)
+    if code is None:
+        raise ValueError(f"x: float32, float16 or bfloat16 is wanted, got {x.dtype}")
     if not x.is_cuda:
-        raise _lib.FisrError(f"{what} is on {x.device}: a GPU tensor is wanted (there is no CPU fallback)")
+        raise _lib.FisrError(f"x is on {x.device}: a GPU tensor is wanted (there is no CPU fallback)")
+    return code, x.get_device()
 
 
-def _like(t, x, what, dtype=None):
-    if t.shape != x.shape or t.dtype != x.dtype or t.device != x.device:
+def _images(x, groups):
+    shape = x.shape
+    if len(shape) != 4:
+        raise ValueError(f"x: [N, H, W, C] is wanted, got {tuple(shape)}")
+    if (x.numel() > _INT and max(shape) > _INT) or not -1 <= groups <= _INT:
+        raise ValueError(f"x: {tuple(shape)} in {groups} groups: a size is too large")
+    return shape
+
+
+def _like(t, x, dev, what):
+    if t.shape != x.shape or t.dtype != x.dtype or t.get_device() != dev:
         raise ValueError(f"{what}: {tuple(t.shape)} {t.dtype} on {t.device} does not fit {tuple(x.shape)} {x.dtype} on {x.device}")
     return t
 
 
-def _param(t, x, shape, what):
+def _param(t, dev, shape, what):
     if t is None:
         return None
-    if t.shape != shape or t.dtype != torch.float32 or t.device != x.device or not t.is_contiguous():
-        raise ValueError(f"{what}: a dense float32 tensor {tuple(shape)} on {x.device} is wanted, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    if t.shape != shape or t.dtype != torch.float32 or t.get_device() != dev or not t.is_contiguous():
+        raise ValueError(f"{what}: a dense float32 tensor {tuple(shape)} on GPU {dev} is wanted, got {tuple(t.shape)} {t.dtype} on {t.device}")
     return t.data_ptr()
 
 
@@ -95,35 +114,46 @@ def _act(act):
         raise ValueError(f"act: one of {', '.join(ACTIVATIONS)} is wanted, got {act!r}") from None
 
 
-def _drop(dropout, x):
+def _drop(dropout, dev):
     if dropout is None:
         return None
-    if dropout.counter is not None and dropout.counter.device != x.device:
-        raise ValueError(f"dropout: the counter is on {dropout.counter.device}, the tensor on {x.device}")
+    if dropout.counter is not None and dropout.counter.get_device() != dev:
+        raise ValueError(f"dropout: the counter is on {dropout.counter.device}, the tensor on GPU {dev}")
     return dropout.desc
 
 
-def _stream(x):
-    return torch._C._cuda_getCurrentRawStream(x.device.index)
+_stream = torch._C._cuda_getCurrentRawStream          # of a device's index: torch.cuda.current_stream(...).cuda_stream without the object
 
 
-def _workspace(L, x, n, h, w, c, groups, backward):
-    nbytes = L.fisr_train_groupnorm_workspace_bytes(n, h, w, c, groups, backward)
-    return (torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None), nbytes
+def _out(x, out, cs, dev, what):
+    """The output tensor and its pixel stride."""
+    if out is not None:
+        return _like(out, x, dev, what), _pixel_stride(out, what)
+    if cs == x.shape[3] and x.is_contiguous():
+        return torch.empty_like(x), cs
+    return x.new_empty(x.shape), x.shape[3]
+
+
+def _workspace(x, n, h, w, c, groups, backward):
+    nbytes = _fn.ws_bytes(n, h, w, c, groups, backward)
+    return x.new_empty(nbytes, dtype=torch.uint8), nbytes
 
 
 def group_norm(x, groups, gamma=None, beta=None, *, eps=1e-5, act="none", dropout=None, out=None):
     """drop(act((x - mean) * rstd * gamma + beta)) with the mean and rstd = 1 / sqrt(var + eps) of every image's groups of channels.
     Returns (y, stats), stats [2, N, groups] float32: means and rstd, what group_norm_backward takes.  `out` may be x."""
-    _images(x, "x", groups)
-    n, h, w, c = x.shape
-    L = _lib.lib()
-    y = torch.empty((n, h, w, c), dtype=x.dtype, device=x.device) if out is None else _like(out, x, "out")
-    stats = torch.empty((2, n, groups), dtype=torch.float32, device=x.device) if groups > 0 else None
-    ws, nbytes = _workspace(L, x, n, h, w, c, groups, 0)
-    _check(L.fisr_train_groupnorm(x.data_ptr(), _pixel_stride(x, "x"), _param(gamma, x, (c,), "gamma"), _param(beta, x, (c,), "beta"),
-                                  y.data_ptr(), _pixel_stride(y, "out"), stats.data_ptr() if stats is not None else None, n, h, w, c, groups, eps, _act(act), _drop(dropout, x),
-                                  _TYPES[x.dtype], ws.data_ptr() if nbytes else None, nbytes, _stream(x)))
+    n, h, w, c = _images(x, groups)
+    code, dev = _type(x)
+    x_cs = _pixel_stride(x, "x")
+    y, y_cs = _out(x, out, x_cs, dev, "out")
+    stats = x.new_empty((2, n, max(groups, 0)), dtype=torch.float32)
+    g, b, a, d, st = _param(gamma, dev, (c,), "gamma"), _param(beta, dev, (c,), "beta"), _act(act), _drop(dropout, dev), _stream(dev)
+    rc = _fn.gn(x.data_ptr(), x_cs, g, b, y.data_ptr(), y_cs, stats.data_ptr(), n, h, w, c, groups, eps, a, d, code, None, 0, st)
+    if rc == _ENOMEM:                                  # a tensor that one launch does not hold
+        ws, nbytes = _workspace(x, n, h, w, c, groups, 0)
+        rc = _fn.gn(x.data_ptr(), x_cs, g, b, y.data_ptr(), y_cs, stats.data_ptr(), n, h, w, c, groups, eps, a, d, code, ws.data_ptr(), nbytes, st)
+    if rc < 0:
+        _lib.check(rc)
     return y, stats
 
 
@@ -132,37 +162,37 @@ def group_norm_backward(dy, x, stats, groups, gamma=None, beta=None, *, act="non
     """Gradients of group_norm: (dx, dgamma, dbeta) from dy, the forward pass' x and stats and the same parameters, activation and
     dropout.  dgamma and dbeta (float32 [C]) are made where they are not given; given ones are overwritten or, with `accumulate`, added
     to.  `dx` may be dy."""
-    _images(x, "x", groups)
-    _like(dy, x, "dy")
-    n, h, w, c = x.shape
-    L = _lib.lib()
-    dx = torch.empty((n, h, w, c), dtype=x.dtype, device=x.device) if dx is None else _like(dx, x, "dx")
+    n, h, w, c = _images(x, groups)
+    code, dev = _type(x)
+    _like(dy, x, dev, "dy")
+    x_cs = _pixel_stride(x, "x")
+    dx, dx_cs = _out(x, dx, x_cs, dev, "dx")
     if accumulate and (dgamma is None or dbeta is None):
         raise ValueError("accumulate: dgamma and dbeta have to be given")
-    dgamma = torch.empty(c, dtype=torch.float32, device=x.device) if dgamma is None else dgamma
-    dbeta = torch.empty(c, dtype=torch.float32, device=x.device) if dbeta is None else dbeta
-    ws, nbytes = _workspace(L, x, n, h, w, c, groups, 1)
-    _check(L.fisr_train_groupnorm_bwd(x.data_ptr(), _pixel_stride(x, "x"), dy.data_ptr(), _pixel_stride(dy, "dy"), _param(gamma, x, (c,), "gamma"),
-                                      _param(beta, x, (c,), "beta"), _param(stats, x, (2, n, groups), "stats"), dx.data_ptr(),
-                                      _pixel_stride(dx, "dx"), _param(dgamma, x, (c,), "dgamma"), _param(dbeta, x, (c,), "dbeta"),
-                                      1 if accumulate else 0, n, h, w, c, groups, _act(act), _drop(dropout, x), _TYPES[x.dtype],
-                                      ws.data_ptr() if nbytes else None, nbytes, _stream(x)))
+    if dgamma is None:
+        dgamma = x.new_empty(c, dtype=torch.float32)
+    if dbeta is None:
+        dbeta = x.new_empty(c, dtype=torch.float32)
+    ws, nbytes = _workspace(x, n, h, w, c, groups, 1)
+    rc = _fn.gn_bwd(x.data_ptr(), x_cs, dy.data_ptr(), _pixel_stride(dy, "dy"), _param(gamma, dev, (c,), "gamma"), _param(beta, dev, (c,), "beta"),
+                    _param(stats, dev, (2, n, groups), "stats"), dx.data_ptr(), dx_cs, _param(dgamma, dev, (c,), "dgamma"),
+                    _param(dbeta, dev, (c,), "dbeta"), 1 if accumulate else 0, n, h, w, c, groups, _act(act), _drop(dropout, dev), code,
+                    ws.data_ptr(), nbytes, _stream(dev))
+    if rc < 0:
+        _lib.check(rc)
     return dx, dgamma, dbeta
 
 
 def dropout(x, drop, residual=None, out=None):
     """drop(x) [+ residual] on a dense tensor of any shape.  `out` may be x or residual."""
-    if x.dtype not in _TYPES:
-        raise ValueError(f"x: float32, float16 or bfloat16 is wanted, got {x.dtype}")
-    if not x.is_cuda:
-        raise _lib.FisrError(f"x is on {x.device}: a GPU tensor is wanted (there is no CPU fallback)")
-    y = torch.empty_like(x, memory_format=torch.contiguous_format) if out is None else _like(out, x, "out")
-    if residual is not None:
-        _like(residual, x, "residual")
-    if not (x.is_contiguous() and y.is_contiguous() and (residual is None or residual.is_contiguous())):
+    code, dev = _type(x)
+    y = torch.empty_like(x) if out is None else _like(out, x, dev, "out")
+    if not (x.is_contiguous() and (out is None or out.is_contiguous()) and (residual is None or residual.is_contiguous())):
         raise ValueError("dropout: dense tensors are wanted (the mask goes by an element's place in one)")
-    _check(_lib.lib().fisr_train_dropout(x.data_ptr(), residual.data_ptr() if residual is not None else None, y.data_ptr(), x.numel(),
-                                         _drop(drop, x), _TYPES[x.dtype], _stream(x)))
+    res = _like(residual, x, dev, "residual").data_ptr() if residual is not None else None
+    rc = _fn.drop(x.data_ptr(), res, y.data_ptr(), x.numel(), _drop(drop, dev), code, _stream(dev))
+    if rc < 0:
+        _lib.check(rc)
     return y
 
 

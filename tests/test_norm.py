@@ -68,7 +68,7 @@ def _drop(p, counter=None):
 
 
 BAD = [dict(x=None), dict(st=None), dict(n=0), dict(h=0), dict(w=-1), dict(c=0), dict(g=0), dict(g=3), dict(x_cs=7), dict(x_cs=-8), dict(act=4), dict(act=-1),
-       dict(type=3), dict(type=-1), dict(ws=None), dict(ws=P + 4), dict(x=P + 2), dict(x=P + 1, type=1), dict(gamma=P + 2), dict(st=P + 1),
+       dict(type=3), dict(type=-1), dict(ws=P + 4), dict(x=P + 2), dict(x=P + 1, type=1), dict(gamma=P + 2), dict(st=P + 1),
        dict(h=1 << 15, w=(1 << 15) + 1), dict(n=(1 << 20) + 1), dict(n=1 << 20, g=8), dict(c=(1 << 16) + 2, x_cs=1 << 17),
        dict(drop=_drop(-0.1)), dict(drop=_drop(1.1)), dict(drop=_drop(float("nan"))), dict(drop=_drop(0.5, P + 4))]
 
@@ -93,6 +93,8 @@ def test_workspace_of_the_wrong_size_is_refused():
     assert 0 < need[0] < need[1]
     assert L.fisr_train_groupnorm_workspace_bytes(0, 2, 2, 8, 2, 0) == 0 and L.fisr_train_groupnorm_workspace_bytes(1, 2, 2, 8, 3, 0) == 0
     assert _gn(n=2, h=200, w=300, c=24, g=4, x_cs=24, y_cs=24, nb=need[0] - 1) == -5
+    assert _gn(n=2, h=200, w=300, c=24, g=4, x_cs=24, y_cs=24, ws=None) == -5
+    assert _gb(ws=None) == -5
     assert _gb(n=2, h=200, w=300, c=24, g=4, x_cs=24, dy_cs=24, dx_cs=24, nb=need[1] - 1) == -5
 
 
