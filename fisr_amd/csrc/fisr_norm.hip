@@ -66,6 +66,10 @@ void set_team(NormArgs& a, int v, int threads, int span) {
   const int groups = span / a.d;
   for (a.jl = 6; a.jl > 0 && groups > threads >> a.jl;) --a.jl;
 }
+// Whether a thread's offset within `rows` pixels may pass 32 bits (see Walk).
+bool wide_strides(const NormArgs& a, int rows, int elem_bytes) {
+  return (unsigned long long)std::max({a.xcs, a.ycs, a.dycs}) * rows * elem_bytes > (1u << 31);
+}
 // lcm(d, v): the least channels that are whole groups and whole vectors
 int span_unit(const NormArgs& a, int v) {
   int unit = a.d;
@@ -78,9 +82,9 @@ struct TeamVariant { int threads, r; };
 constexpr TeamVariant TEAM[] = {{256, 1}, {256, 2}, {256, 4}, {256, 9}, {512, 9}};
 int team_variant(NormArgs& a, int v, int elem_bytes, bool backward) {
   const size_t elems = (size_t)a.n * a.p * a.c;
-  if (elems > (size_t)env_int("NORM_TEAM_K", 16384) << 10) return -1;
+  if (elems > (size_t)env_int("NORM_TEAM_K", 16384) << 10 || wide_strides(a, 512, elem_bytes)) return -1;
   const int unit = span_unit(a, v), most = a.c / unit;
-  const int line = elems * elem_bytes > (size_t)4 << 20 ? 64 : 16;  // least bytes of a span: narrow ones read a cache line many times over
+  const int line = env_int("NORM_LINE", elems * elem_bytes > (size_t)4 << 20 ? 64 : 16);  // least bytes of a span: narrow ones read a cache line many times over
   int best = -1, best_span = 0;
   for (int k = 1; k <= most; ++k) {
     if (most % k) continue;
@@ -103,10 +107,12 @@ int team_variant(NormArgs& a, int v, int elem_bytes, bool backward) {
 }
 template <typename T, int V> void launch_team(const NormArgs& a, bool backward, hipStream_t st) {
   const dim3 grid(a.n * (a.c / a.span));
+  const bool whole = a.slots == 1;
 #define NORM_TEAM(I)                                                                                                                         \
   case I:                                                                                                                                    \
-    if (backward) hipLaunchKernelGGL((norm_team_grad_kernel<T, V, TEAM[I].r, TEAM[I].threads>), grid, dim3(TEAM[I].threads), 0, st, a);       \
-    else hipLaunchKernelGGL((norm_team_kernel<T, V, TEAM[I].r, TEAM[I].threads>), grid, dim3(TEAM[I].threads), 0, st, a);                     \
+    if (!backward) hipLaunchKernelGGL((norm_team_kernel<T, V, TEAM[I].r, TEAM[I].threads>), grid, dim3(TEAM[I].threads), 0, st, a);           \
+    else if (whole) hipLaunchKernelGGL((norm_team_grad_kernel<T, V, TEAM[I].r, TEAM[I].threads, true>), grid, dim3(TEAM[I].threads), 0, st, a);\
+    else hipLaunchKernelGGL((norm_team_grad_kernel<T, V, TEAM[I].r, TEAM[I].threads, V == 1>), grid, dim3(TEAM[I].threads), 0, st, a);         \
     break;
   switch (a.team) { NORM_TEAM(0) NORM_TEAM(1) NORM_TEAM(2) NORM_TEAM(3) NORM_TEAM(4) }
 #undef NORM_TEAM
@@ -115,6 +121,7 @@ template <typename T, int V> void launch_team(const NormArgs& a, bool backward, 
 
 // Two launches over chunks of pixels: grids and the channels of a workgroup (all, or the most whole groups that it has threads for).
 bool two_tiling(NormArgs& a, int v, int elem_bytes, bool backward) {
+  if (wide_strides(a, 256, elem_bytes)) return false;
   const int unit = span_unit(a, v), most = a.c / unit;
   int k = most;
   while (k > 0 && (most % k || k * unit / v > 256)) --k;
@@ -122,34 +129,35 @@ bool two_tiling(NormArgs& a, int v, int elem_bytes, bool backward) {
   set_team(a, v, 256, k * unit);
   // first launch: long-lived workgroups (their numbers have to be joined); second: some 48 KB each, four a CU at least
   const size_t bytes = (size_t)a.n * a.p * a.c * elem_bytes * (backward ? 2 : 1);
-  chunks_for(a, env_int("NORM_SWG", bytes > (size_t)128 << 20 ? 1024 : 512), a.chunks, a.ppc);
+  chunks_for(a, env_int("NORM_SWG", backward && elem_bytes == 4 ? 1024 : 512), a.chunks, a.ppc);
   chunks_for(a, env_int("NORM_AWG", (int)std::min<size_t>(std::max<size_t>(bytes / 49152, 1024), 16384)), a.achunks, a.appc);
   return true;
 }
-template <typename T, int V, bool NT> void launch_two_nt(NormArgs a, bool backward, hipStream_t st) {
+template <typename T, int V, bool WHOLE> void launch_two_whole(const NormArgs& a, bool backward, hipStream_t st) {
   constexpr int TH = 256;
   const int ny = a.c / a.span;
   const dim3 g1(a.n * a.chunks, ny);
   if (backward) {
     const int pblocks = a.dgamma || a.dbeta ? (a.c + 15) / 16 : 0;
-    hipLaunchKernelGGL((norm_chunk_sums_kernel<T, V, TH, NT>), g1, dim3(TH), 0, st, a);
-    hipLaunchKernelGGL((norm_chunk_grad_kernel<T, V, TH, NT>), dim3(pblocks + a.n * a.achunks, ny), dim3(TH), 0, st, a, pblocks);
+    hipLaunchKernelGGL((norm_chunk_sums_kernel<T, V, TH, WHOLE>), g1, dim3(TH), 0, st, a);
+    hipLaunchKernelGGL((norm_chunk_grad_kernel<T, V, TH, WHOLE>), dim3(pblocks + a.n * a.achunks, ny), dim3(TH), 0, st, a, pblocks);
     return;
   }
   const int join = a.chunks * (a.span / a.d) <= env_int("NORM_JOIN", 2048);
-  hipLaunchKernelGGL((norm_chunk_stats_kernel<T, V, TH, NT>), g1, dim3(TH), 0, st, a);
+  hipLaunchKernelGGL((norm_chunk_stats_kernel<T, V, TH>), g1, dim3(TH), 0, st, a);
   if (!join) {
     NormArgs b = a;
     b.jl = 6;
     hipLaunchKernelGGL(norm_join_kernel, dim3(a.n * a.groups), dim3(64), 0, st, b);
   }
-  hipLaunchKernelGGL((norm_chunk_apply_kernel<T, V, TH, NT>), dim3(a.n * a.achunks, ny), dim3(TH), 0, st, a, join);
+  hipLaunchKernelGGL((norm_chunk_apply_kernel<T, V, TH, WHOLE>), dim3(a.n * a.achunks, ny), dim3(TH), 0, st, a, join);
 }
 template <typename T, int V> bool launch_two(NormArgs a, bool backward, hipStream_t st) {
   if (!two_tiling(a, V, sizeof(T), backward)) return false;
   const size_t bytes = (size_t)a.n * a.p * a.c * sizeof(T) * (backward ? 2 : 1);
-  if (bytes > (size_t)env_int("NORM_NT_MB", 128) << 20) launch_two_nt<T, V, true>(a, backward, st);
-  else launch_two_nt<T, V, false>(a, backward, st);
+  a.nt = bytes > (size_t)env_int("NORM_NT_MB", 128) << 20;
+  if (a.slots == 1) launch_two_whole<T, V, true>(a, backward, st);
+  else launch_two_whole<T, V, V == 1>(a, backward, st);
   return true;
 }
 
@@ -215,7 +223,7 @@ int norm_call(const char* who, NormArgs& a, bool backward, int n, int h, int w, 
     return bad("a pointer is not aligned to its element");
   if (act < FISR_ACT_NONE || act > FISR_ACT_GELU) return bad("unknown activation");
   if (const char* e = drop_error(drop, a.drop)) return bad(e);
-  a.n = n; a.p = h * w; a.c = c; a.groups = groups; a.d = c / groups; a.by_d = magic(a.d); a.act = act;
+  a.n = n; a.p = h * w; a.c = c; a.groups = groups; a.d = c / groups; a.by_d = magic(a.d); a.act = act; a.inv_m = (float)(1.0 / ((double)a.p * a.d));
   a.mean = mean_rstd; a.rstd = mean_rstd + (size_t)n * groups;
   if ((uintptr_t)ws % 16) return bad("the workspace is not aligned to 16 bytes");
   a.team = team_variant(a, es == 4 ? norm_vec<float>(a) : norm_vec<f16_t>(a), (int)es, backward);

@@ -13,6 +13,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace fisr {
 
 typedef _Float16 f16_t;
@@ -68,81 +70,93 @@ template <int V> __device__ __forceinline__ void drop_apply(float (&v)[V], uint6
   }
 }
 
-// ---- loads and stores of V channels as floats.  The caller sees to alignment: 16 bytes, or V elements where that is less ----
-template <typename T, int V> struct alignas(sizeof(T) * V < 16 ? sizeof(T) * V : 16) Pack { T e[V]; };
-template <typename T, int V> __device__ __forceinline__ void load_v(const T* p, float (&v)[V]) {
-  const Pack<T, V> q = *reinterpret_cast<const Pack<T, V>*>(p);
+// ---- vectors of V channels as they lie in memory.  The caller sees to alignment: 16 bytes, or V elements where that is less ----
+// Two and more 16-bit elements are kept as 32-bit words: as an array of elements the compiler takes a loaded vector apart and joins it again.
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+template <typename T, int V> struct alignas(sizeof(T) * V < 16 ? sizeof(T) * V : 16) Pack {
+  static constexpr bool WORDS = sizeof(T) * V >= 4;
+  typedef typename std::conditional<WORDS, uint32_t, T>::type E;
+  static constexpr int N = sizeof(T) * V / sizeof(E);
+  E w[N];
+  __device__ __forceinline__ float get(int e) const {
+    if constexpr (!WORDS) return (float)w[e];
+    else if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, w[e]);
+    else if constexpr (std::is_same<T, b16_t>::value) return __builtin_bit_cast(float, e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+    else {
+      struct H { f16_t h[2]; };
+      return (float)__builtin_bit_cast(H, w[e >> 1]).h[e & 1];
+    }
+  }
+  __device__ __forceinline__ void widen(float (&v)[V]) const {
 #pragma unroll
-  for (int e = 0; e < V; ++e) v[e] = (float)q.e[e];
+    for (int e = 0; e < V; ++e) v[e] = get(e);
+  }
+  __device__ __forceinline__ void round(const float (&v)[V]) {
+    if constexpr (!WORDS) w[0] = (T)v[0];
+    else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) w[e] = __builtin_bit_cast(uint32_t, v[e]);
+    } else {
+      struct H { T h[2]; };
+#pragma unroll
+      for (int e = 0; e < V; e += 2) w[e >> 1] = __builtin_bit_cast(uint32_t, H{{(T)v[e], (T)v[e + 1]}});
+    }
+  }
+  __device__ __forceinline__ void load(const T* p) { *this = *reinterpret_cast<const Pack*>(p); }
+  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<Pack*>(p) = *this; }
+  // non-temporal: what is read or written once and is larger than the caches hold
+  __device__ __forceinline__ void load_nt(const T* p) {
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+      for (int k = 0; k < N / 4; ++k) {
+        const u32x4 u = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p) + k);
+        w[4 * k] = u.x; w[4 * k + 1] = u.y; w[4 * k + 2] = u.z; w[4 * k + 3] = u.w;
+      }
+    } else if constexpr (N == 2) {
+      const u32x2 u = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p));
+      w[0] = u.x; w[1] = u.y;
+    } else if constexpr (WORDS) {
+      w[0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p));
+    } else {
+      load(p);
+    }
+  }
+  __device__ __forceinline__ void store_nt(T* p) const {
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+      for (int k = 0; k < N / 4; ++k) __builtin_nontemporal_store(u32x4{w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]}, reinterpret_cast<u32x4*>(p) + k);
+    } else if constexpr (N == 2) {
+      __builtin_nontemporal_store(u32x2{w[0], w[1]}, reinterpret_cast<u32x2*>(p));
+    } else if constexpr (WORDS) {
+      __builtin_nontemporal_store(w[0], reinterpret_cast<uint32_t*>(p));
+    } else {
+      store(p);
+    }
+  }
+  // Hides from the compiler that a register still holds what it held: it would otherwise keep a 16-bit vector's float32 form from one pass over
+  // the registers to the next, at twice the registers.
+  __device__ __forceinline__ void keep() {
+    if constexpr (sizeof(T) == 2 && WORDS) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) asm volatile("" : "+v"(w[e]));
+    }
+  }
+};
+template <typename T, int V> __device__ __forceinline__ void load_v(const T* p, float (&v)[V]) {
+  Pack<T, V> q;
+  q.load(p);
+  q.widen(v);
 }
 template <typename T, int V> __device__ __forceinline__ void store_v(T* p, const float (&v)[V]) {
   Pack<T, V> q;
-#pragma unroll
-  for (int e = 0; e < V; ++e) q.e[e] = (T)v[e];
-  *reinterpret_cast<Pack<T, V>*>(p) = q;
-}
-
-template <typename T, int V> __device__ __forceinline__ void widen(const Pack<T, V>& q, float (&v)[V]) {
-#pragma unroll
-  for (int e = 0; e < V; ++e) v[e] = (float)q.e[e];
-}
-// Streaming forms (non-temporal): what is read or written once and is larger than the caches hold.
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-template <typename T, int V> __device__ __forceinline__ Pack<T, V> load_nt(const T* p) {
-  constexpr int B = sizeof(T) * V;
-  Pack<T, V> q;
-  if constexpr (B >= 16) {
-    struct Q { u32x4 w[B / 16]; } u;
-#pragma unroll
-    for (int k = 0; k < B / 16; ++k) u.w[k] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p) + k);
-    q = __builtin_bit_cast(Pack<T, V>, u);
-  } else if constexpr (B == 8) {
-    q = __builtin_bit_cast(Pack<T, V>, __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p)));
-  } else if constexpr (B == 4) {
-    q = __builtin_bit_cast(Pack<T, V>, __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p)));
-  } else {
-    q = *reinterpret_cast<const Pack<T, V>*>(p);
-  }
-  return q;
+  q.round(v);
+  q.store(p);
 }
 template <typename T, int V> __device__ __forceinline__ void store_nt(T* p, const float (&v)[V]) {
-  constexpr int B = sizeof(T) * V;
   Pack<T, V> q;
-#pragma unroll
-  for (int e = 0; e < V; ++e) q.e[e] = (T)v[e];
-  if constexpr (B >= 16) {
-    struct Q { u32x4 w[B / 16]; };
-    const Q u = __builtin_bit_cast(Q, q);
-#pragma unroll
-    for (int k = 0; k < B / 16; ++k) __builtin_nontemporal_store(u.w[k], reinterpret_cast<u32x4*>(p) + k);
-  } else if constexpr (B == 8) {
-    __builtin_nontemporal_store(__builtin_bit_cast(u32x2, q), reinterpret_cast<u32x2*>(p));
-  } else if constexpr (B == 4) {
-    __builtin_nontemporal_store(__builtin_bit_cast(uint32_t, q), reinterpret_cast<uint32_t*>(p));
-  } else {
-    *reinterpret_cast<Pack<T, V>*>(p) = q;
-  }
-}
-template <bool NT, typename T, int V> __device__ __forceinline__ Pack<T, V> load_p(const T* p) {
-  if constexpr (NT) return load_nt<T, V>(p);
-  else return *reinterpret_cast<const Pack<T, V>*>(p);
-}
-template <bool NT, typename T, int V> __device__ __forceinline__ void store_p(T* p, const float (&v)[V]) {
-  if constexpr (NT) store_nt<T, V>(p, v);
-  else store_v<T, V>(p, v);
-}
-
-// Hides from the compiler that a register still holds what it held: it would otherwise keep a 16-bit vector's float32 form from one pass
-// over the registers to the next, at twice the registers (18 vectors a thread spill then).
-template <typename T, int V> __device__ __forceinline__ void keep_packed(Pack<T, V>& q) {
-  if constexpr (sizeof(T) == 2 && V % 2 == 0) {
-    struct Words { uint32_t w[V / 2]; };
-    Words u = __builtin_bit_cast(Words, q);
-#pragma unroll
-    for (int e = 0; e < V / 2; ++e) asm volatile("" : "+v"(u.w[e]));
-    q = __builtin_bit_cast(Pack<T, V>, u);
-  }
+  q.round(v);
+  q.store_nt(p);
 }
 
 // ---- activations ----
@@ -177,9 +191,9 @@ template <int V> __device__ __forceinline__ void act_grad_apply(float (&g)[V], c
     for (int e = 0; e < V; ++e) { const float s = sigmoid_f(z[e]); g[e] *= s * (1.f + z[e] * (1.f - s)); }
   } else if (act == NORM_ACT_GELU) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const float n = gauss_f(z[e]), q = phi_tail(z[e], n);
-      g[e] *= (z[e] < 0.f ? q : 1.f - q) + z[e] * (0.39894228f * n);
+    for (int e = 0; e < V; ++e) {                              // Phi = 1/2 + sign(z) (1/2 - Phi(-|z|))
+      const float n = gauss_f(z[e]), half = copysignf(0.5f - phi_tail(z[e], n), z[e]);
+      g[e] *= 0.5f + (half + z[e] * (0.39894228f * n));
     }
   }
 }
@@ -200,7 +214,9 @@ struct NormArgs {
   int achunks, appc;                                   // ... in the second of two launches
   int slots, per_group, jl;                            // see team_sums
   uint32_t by_d, by_cb, by_rows, by_per_group;               // for div_by
-  float eps; int act, accumulate, team;                // team: the host's variant of the one-launch form
+  float eps, inv_m;                                    // inv_m: 1 / (p * d)
+  int act, accumulate;
+  int team, nt;                                        // the host's variant of the one-launch form; whether reads pass the caches
   DropArgs drop;
 };
 // x / y for x < 2^16 and y <= 2^16 by the host's ceil(2^32 / y) (0 for y = 1): a division by a number of the launch is some 20 instructions
@@ -220,7 +236,7 @@ template <int V> __device__ __forceinline__ void team_threads(NormTeam& t, const
   t.on = t.row < a.rows;
 }
 
-// ---- sums over a workgroup's pixels and the channels of each of its groups: tot[group], seen by every thread.  All threads call. ----
+// ---- sums over a workgroup's pixels and the channels of each of its groups: tot[group] = last(sum), seen by every thread.  All threads call. ----
 // A thread first adds the channels of its vector that share a group (slots numbers are left: 1, V / d or V), a wave its rows where columns
 // are a power of two, then 2^jl lanes a group add what is left of all groups at once.  `red`: TH * V floats.
 template <int V> __device__ __forceinline__ int fold_slots(const NormArgs& a, float (&v)[V]) {
@@ -234,7 +250,7 @@ template <int V> __device__ __forceinline__ int fold_slots(const NormArgs& a, fl
   }
   return a.slots;
 }
-template <int V, int TH> __device__ __forceinline__ void team_sums(const NormArgs& a, const NormTeam& t, float (&v)[V], float* red, float* tot) {
+template <int V, int TH, typename F> __device__ __forceinline__ void team_sums(const NormArgs& a, const NormTeam& t, float (&v)[V], float* red, float* tot, F last) {
   const int slots = fold_slots<V>(a, v), per_row = a.cb * slots;
   const bool pow2 = a.cb <= 64 && (a.cb & (a.cb - 1)) == 0;
   int rows = a.rows;
@@ -260,7 +276,7 @@ template <int V, int TH> __device__ __forceinline__ void team_sums(const NormArg
     if (j < groups)
       for (int i = lane; i < total; i += lanes) { const int q = div_by(i, a.by_per_group); s += red[q * per_row + j * a.per_group + (i - q * a.per_group)]; }
     for (int k = lanes >> 1; k; k >>= 1) s += __shfl_xor(s, k);
-    if (j < groups && lane == 0) tot[j] = s;
+    if (j < groups && lane == 0) tot[j] = last(s);
   }
   __syncthreads();
 }
@@ -281,17 +297,37 @@ template <int V> __device__ __forceinline__ NormTeam span_team(const NormArgs& a
   return t;
 }
 
+// A thread's vectors of one tensor: number r is r * step bytes from its first.  The launch's part of an address stays in scalar registers
+// (base, r * step), the thread's is a 32-bit offset (the host sees to that), so a load costs no vector instruction beside itself.
+template <typename T, int V> struct Walk {
+  char* base;
+  uint32_t at;
+  size_t step;
+  __device__ __forceinline__ Walk(const NormArgs& a, const NormTeam& t, const void* x, size_t cs, int p0)
+      : base((char*)x + (((size_t)t.img * a.p + p0) * cs + t.cbase) * sizeof(T)), at((uint32_t)((t.row * (uint32_t)cs + t.col * V) * sizeof(T))),
+        step(a.rows * cs * sizeof(T)) {}
+  __device__ __forceinline__ T* ptr(int r) const { return reinterpret_cast<T*>(base + (size_t)r * step + at); }
+  template <int U> __device__ __forceinline__ void load(Pack<T, V> (&q)[U], int r, int m, int nt) const {      // nt: past the caches
+    if (nt) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (u < m) q[u].load_nt(ptr(r + u));
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (u < m) q[u].load(ptr(r + u));
+    }
+  }
+};
 template <typename T, int V, int R, int TH> __global__ __launch_bounds__(TH) void norm_team_kernel(const NormArgs a) {
   __shared__ float red[TH * V];
   __shared__ float tot[2][TH * V];                           // (as many groups as channels at the most)
   const NormTeam t = span_team<V>(a);
-  const T* x = (const T*)a.x + (size_t)t.img * a.p * a.xcs + t.c0;
+  const Walk<T, V> x(a, t, a.x, a.xcs, 0), y(a, t, a.y, a.ycs, 0);
   Pack<T, V> q[R];
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int p = t.row + r * a.rows;
-    if (t.on && p < a.p) q[r] = *reinterpret_cast<const Pack<T, V>*>(x + (size_t)p * a.xcs);
-  }
+  for (int r = 0; r < R; ++r)
+    if (t.on && t.row + r * a.rows < a.p) q[r].load(x.ptr(r));
   float gamma[V], beta[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) {
@@ -305,46 +341,43 @@ template <typename T, int V, int R, int TH> __global__ __launch_bounds__(TH) voi
   for (int r = 0; r < R; ++r)
     if (t.on && t.row + r * a.rows < a.p) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) s[e] += (float)q[r].e[e];
+      for (int e = 0; e < V; ++e) s[e] += q[r].get(e);
     }
-  team_sums<V, TH>(a, t, s, red, tot[0]);
+  team_sums<V, TH>(a, t, s, red, tot[0], [&](float v) { return v * a.inv_m; });
 #pragma unroll
-  for (int r = 0; r < R; ++r) keep_packed<T, V>(q[r]);
-  const float inv = 1.f / ((float)a.p * (float)a.d);
+  for (int r = 0; r < R; ++r) q[r].keep();
   float mean[V];
 #pragma unroll
-  for (int e = 0; e < V; ++e) { mean[e] = t.on ? tot[0][div_by(t.col * V + e, a.by_d)] * inv : 0.f; s[e] = 0.f; }
+  for (int e = 0; e < V; ++e) { mean[e] = t.on ? tot[0][div_by(t.col * V + e, a.by_d)] : 0.f; s[e] = 0.f; }
 #pragma unroll
   for (int r = 0; r < R; ++r)
     if (t.on && t.row + r * a.rows < a.p) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) { const float dv = (float)q[r].e[e] - mean[e]; s[e] += dv * dv; }
+      for (int e = 0; e < V; ++e) { const float dv = q[r].get(e) - mean[e]; s[e] += dv * dv; }
     }
-  team_sums<V, TH>(a, t, s, red, tot[1]);
+  team_sums<V, TH>(a, t, s, red, tot[1], [&](float v) { return inv_std(v * a.inv_m, a.eps); });
 #pragma unroll
-  for (int r = 0; r < R; ++r) keep_packed<T, V>(q[r]);
+  for (int r = 0; r < R; ++r) q[r].keep();
   for (int j = threadIdx.x; j < a.span / a.d; j += TH) {
     const size_t g = (size_t)t.img * a.groups + t.cbase / a.d + j;
-    a.mean[g] = tot[0][j] * inv;
-    a.rstd[g] = inv_std(tot[1][j] * inv, a.eps);
+    a.mean[g] = tot[0][j];
+    a.rstd[g] = tot[1][j];
   }
   if (!t.on) return;
 #pragma unroll
-  for (int e = 0; e < V; ++e) gamma[e] *= inv_std(tot[1][div_by(t.col * V + e, a.by_d)] * inv, a.eps);
+  for (int e = 0; e < V; ++e) gamma[e] *= tot[1][div_by(t.col * V + e, a.by_d)];
   const uint64_t offset = a.drop.thresh ? drop_offset(a.drop) : 0;
-  T* y = (T*)a.y + (size_t)t.img * a.p * a.ycs + t.c0;
+  const uint64_t i0 = ((uint64_t)t.img * a.p + t.row) * a.c + t.c0, di = (uint64_t)a.rows * a.c;
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int p = t.row + r * a.rows;
-    if (p < a.p) {
+  for (int r = 0; r < R; ++r)
+    if (t.row + r * a.rows < a.p) {
       float v[V];
 #pragma unroll
-      for (int e = 0; e < V; ++e) v[e] = ((float)q[r].e[e] - mean[e]) * gamma[e] + beta[e];
+      for (int e = 0; e < V; ++e) v[e] = (q[r].get(e) - mean[e]) * gamma[e] + beta[e];
       act_apply<V>(v, a.act);
-      if (a.drop.thresh) drop_apply<V>(v, ((uint64_t)t.img * a.p + p) * a.c + t.c0, a.drop, offset);
-      store_v<T, V>(y + (size_t)p * a.ycs, v);
+      if (a.drop.thresh) drop_apply<V>(v, i0 + r * di, a.drop, offset);
+      store_v<T, V>(y.ptr(r), v);
     }
-  }
 }
 
 // ---- two launches, one read each: statistics per group and chunk of pixels, then the output ----
@@ -364,7 +397,7 @@ template <int V> __device__ __forceinline__ NormTeam chunk_team(const NormArgs& 
 // Chan's formula, so nothing is lost when the mean is large against the spread: no sum of squares about a far point exists anywhere.
 template <typename T, int V, int U> __device__ __forceinline__ void stats_batch(Pack<T, V> (&q)[U], int m, float (&mean)[V], float (&m2)[V], float& cnt) {
   float bm[V], b2[V];
-  const float fm = (float)m, im = 1.f / fm, w = fm / (cnt + fm), nw = cnt * w;
+  const float fm = (float)m, im = __builtin_amdgcn_rcpf(fm), w = fm * __builtin_amdgcn_rcpf(cnt + fm), nw = cnt * w;      // (1 / 4 is exact)
   cnt += fm;
 #pragma unroll
   for (int e = 0; e < V; ++e) bm[e] = b2[e] = 0.f;
@@ -372,24 +405,52 @@ template <typename T, int V, int U> __device__ __forceinline__ void stats_batch(
   for (int u = 0; u < U; ++u)
     if (u < m) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) bm[e] += (float)q[u].e[e];
+      for (int e = 0; e < V; ++e) bm[e] += q[u].get(e);
     }
 #pragma unroll
   for (int e = 0; e < V; ++e) bm[e] *= im;
 #pragma unroll
-  for (int u = 0; u < U; ++u) keep_packed<T, V>(q[u]);
+  for (int u = 0; u < U; ++u) q[u].keep();
 #pragma unroll
   for (int u = 0; u < U; ++u)
     if (u < m) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) { const float dv = (float)q[u].e[e] - bm[e]; b2[e] += dv * dv; }
+      for (int e = 0; e < V; ++e) { const float dv = q[u].get(e) - bm[e]; b2[e] += dv * dv; }
     }
 #pragma unroll
   for (int e = 0; e < V; ++e) { const float dm = bm[e] - mean[e]; mean[e] += dm * w; m2[e] += b2[e] + dm * dm * nw; }
 }
 
-template <typename T, int V, int TH, bool NT> __global__ __launch_bounds__(TH) void norm_chunk_stats_kernel(const NormArgs a) {
+// The vectors of a thread in a chunk, U at a time, the next ones on their way while these are worked on: two buffers in turn (a copy between
+// them would cost as many instructions as a vector's arithmetic).  `load(buffer, r, m)` and `work(buffer, r, m)` take vectors r .. r + m - 1;
+// m is U but for the last ones.  begin() loads the first, finish() does the rest.
+template <int U, typename B> struct Chunk {
+  int full, tail;
+  B b0, b1;
+  __device__ __forceinline__ Chunk(const NormArgs& a, const NormTeam& t, int len) {
+    full = len / (U * a.rows);                               // the same for every thread
+    const int left = len - full * U * a.rows - t.row;
+    tail = left > 0 ? div_by(left + a.rows - 1, a.by_rows) : 0;
+  }
+  template <typename L> __device__ __forceinline__ void fetch(B& b, int k, L load) { k < full ? load(b, k * U, U) : load(b, k * U, tail); }
+  template <typename L, typename W> __device__ __forceinline__ void finish(L load, W work) {
+    int k = 0;
+    while (k < full) {
+      fetch(b1, k + 1, load);
+      work(b0, k * U, U);
+      if (++k == full) { b0 = b1; break; }
+      fetch(b0, k + 1, load);
+      work(b1, k * U, U);
+      ++k;
+    }
+    work(b0, full * U, tail);
+  }
+};
+
+template <typename T, int V, int U> struct Batch { Pack<T, V> x[U]; };
+template <typename T, int V, int TH> __global__ __launch_bounds__(TH, 4) void norm_chunk_stats_kernel(const NormArgs a) {
   constexpr int U = 4;
+  typedef Batch<T, V, U> B;
   __shared__ float red[TH * V];
   __shared__ float tot[2][TH * V];
   int chunk, p0, p1;
@@ -398,42 +459,22 @@ template <typename T, int V, int TH, bool NT> __global__ __launch_bounds__(TH) v
 #pragma unroll
   for (int e = 0; e < V; ++e) mean[e] = m2[e] = 0.f;
   if (t.on) {
-    const size_t step = (size_t)a.rows * a.xcs;
-    const T* x = (const T*)a.x + ((size_t)t.img * a.p + p0 + t.row) * a.xcs + t.c0;
-    const int batches = (p1 - p0) / (U * a.rows);            // full ones: the same for every thread
-    Pack<T, V> q[U], next[U];
-    if (batches) {
-#pragma unroll
-      for (int u = 0; u < U; ++u) next[u] = load_p<NT, T, V>(x + u * step);
-    }
-    for (int k = 0; k < batches; ++k) {                      // the next batch is on its way while this one is reduced
-#pragma unroll
-      for (int u = 0; u < U; ++u) q[u] = next[u];
-      x += U * step;
-      if (k + 1 < batches) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) next[u] = load_p<NT, T, V>(x + u * step);
-      }
-      stats_batch<T, V, U>(q, U, mean, m2, cnt);
-    }
-    const int left = p1 - (p0 + t.row + batches * U * a.rows), m = left > 0 ? (left + a.rows - 1) / a.rows : 0;
-    if (m) {
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (u < m) q[u] = load_p<NT, T, V>(x + u * step);
-      stats_batch<T, V, U>(q, m, mean, m2, cnt);
-    }
+    const Walk<T, V> x(a, t, a.x, a.xcs, p0);
+    Chunk<U, B> c(a, t, p1 - p0);
+    const auto load = [&](B& b, int r, int m) { x.load(b.x, r, m, a.nt); };
+    c.fetch(c.b0, 0, load);
+    c.finish(load, [&](B& b, int, int m) { if (m) stats_batch<T, V, U>(b.x, m, mean, m2, cnt); });
   }
   float s[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) s[e] = cnt * mean[e];
-  team_sums<V, TH>(a, t, s, red, tot[0]);
   const float inv = 1.f / ((float)(p1 - p0) * (float)a.d);
+  team_sums<V, TH>(a, t, s, red, tot[0], [&](float v) { return v * inv; });
 #pragma unroll
-  for (int e = 0; e < V; ++e) { const float dm = t.on ? mean[e] - tot[0][div_by(t.col * V + e, a.by_d)] * inv : 0.f; s[e] = m2[e] + cnt * dm * dm; }
-  team_sums<V, TH>(a, t, s, red, tot[1]);
+  for (int e = 0; e < V; ++e) { const float dm = t.on ? mean[e] - tot[0][div_by(t.col * V + e, a.by_d)] : 0.f; s[e] = m2[e] + cnt * dm * dm; }
+  team_sums<V, TH>(a, t, s, red, tot[1], [](float v) { return v; });
   for (int j = threadIdx.x; j < a.span / a.d; j += TH)
-    a.part[((size_t)t.img * a.groups + t.cbase / a.d + j) * a.chunks + chunk] = make_float2(tot[0][j] * inv, tot[1][j]);
+    a.part[((size_t)t.img * a.groups + t.cbase / a.d + j) * a.chunks + chunk] = make_float2(tot[0][j], tot[1][j]);
 }
 
 // mean and rstd of `count` groups from the chunks' numbers: 2^jl lanes a group, all groups at once (a wave a group in turn would be two round
@@ -491,28 +532,20 @@ template <int V> __device__ __forceinline__ void drop_apply_pair(float (&v0)[V],
   }
 }
 
-// U pixels of a thread from pixel p on, m of them there
-template <typename T, int V, int U, bool NT> __device__ __forceinline__ void load_batch(Pack<T, V> (&q)[U], const T* base, size_t cs, int rows, int p, int m) {
-  const T* x = base + (size_t)p * cs;
-#pragma unroll
-  for (int u = 0; u < U; ++u)
-    if (u < m) q[u] = load_p<NT, T, V>(x + (size_t)(u * rows) * cs);
-}
-__device__ __forceinline__ int batch_count(const NormArgs& a, const NormTeam& t, int p, int p1) { return t.on && p < p1 ? div_by(min(p1 - p, 65535 - a.rows) + a.rows - 1, a.by_rows) : 0; }
 
-template <typename T, int V, int TH, bool NT> __global__ __launch_bounds__(TH) void norm_chunk_apply_kernel(const NormArgs a, int join) {
-  constexpr int U = 4;
+template <typename T, int V, int TH, bool WHOLE> __global__ __launch_bounds__(TH) void norm_chunk_apply_kernel(const NormArgs a, int join) {
+  constexpr int U = 4, W = WHOLE ? 1 : V;
+  typedef Batch<T, V, U> B;
   __shared__ float mean_s[TH * V], rstd_s[TH * V];
   int chunk, p0, p1;
   const NormTeam t = chunk_team<V>(a, blockIdx.x, a.achunks, a.appc, chunk, p0, p1);
-  const T* x = (const T*)a.x + (size_t)t.img * a.p * a.xcs + t.c0;
-  T* y = (T*)a.y + (size_t)t.img * a.p * a.ycs + t.c0;
-  int p = p0 + t.row, m = batch_count(a, t, p, p1);
-  Pack<T, V> q[U], next[U];
-  load_batch<T, V, U, NT>(q, x, a.xcs, a.rows, p, m);        // on its way while the statistics come
+  const Walk<T, V> x(a, t, a.x, a.xcs, p0), y(a, t, a.y, a.ycs, p0);
+  Chunk<U, B> c(a, t, p1 - p0);
+  const auto load = [&](B& b, int r, int m) { x.load(b.x, r, m, a.nt); };
+  if (t.on) c.fetch(c.b0, 0, load);                          // on its way while the statistics come
   const size_t g0 = (size_t)t.img * a.groups + div_by(t.cbase, a.by_d);
   const float *mg = a.mean + g0, *rg = a.rstd + g0;
-  float mean[V], scale[V], beta[V];
+  float mean[W], scale[V], beta[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) {
     scale[e] = t.on && a.gamma ? a.gamma[t.c0 + e] : 1.f;
@@ -528,16 +561,14 @@ template <typename T, int V, int TH, bool NT> __global__ __launch_bounds__(TH) v
   if (!t.on) return;
 #pragma unroll
   for (int e = 0; e < V; ++e) {
-    const int g = div_by(t.col * V + e, a.by_d);
-    mean[e] = join ? mean_s[g] : mg[g];
+    const int g = div_by(t.col * V + (WHOLE ? 0 : e), a.by_d);
+    if (e < W) mean[e] = join ? mean_s[g] : mg[g];
     scale[e] *= join ? rstd_s[g] : rg[g];
   }
   const uint64_t offset = a.drop.thresh ? drop_offset(a.drop) : 0;
+  const uint64_t i0 = ((uint64_t)t.img * a.p + p0 + t.row) * a.c + t.c0, di = (uint64_t)a.rows * a.c;
   const bool pairs = V == 4 && a.span % 8 == 0;
-  while (m) {
-    const int pn = p + U * a.rows, mn = batch_count(a, t, pn, p1);
-    load_batch<T, V, U, NT>(next, x, a.xcs, a.rows, pn, mn);
-    const uint64_t i = ((uint64_t)t.img * a.p + p) * a.c + t.c0, di = (uint64_t)a.rows * a.c;
+  c.finish(load, [&](B& b, int r, int m) {
 #pragma unroll
     for (int u = 0; u < U; u += 2) {
       float v[2][V];
@@ -545,45 +576,58 @@ template <typename T, int V, int TH, bool NT> __global__ __launch_bounds__(TH) v
       for (int k = 0; k < 2; ++k)
         if (u + k < m) {
 #pragma unroll
-          for (int e = 0; e < V; ++e) v[k][e] = ((float)q[u + k].e[e] - mean[e]) * scale[e] + beta[e];
+          for (int e = 0; e < V; ++e) v[k][e] = (b.x[u + k].get(e) - mean[WHOLE ? 0 : e]) * scale[e] + beta[e];
           act_apply<V>(v[k], a.act);
-          if (a.drop.thresh && !pairs) drop_apply<V>(v[k], i + (u + k) * di, a.drop, offset);
+          if (a.drop.thresh && !pairs) drop_apply<V>(v[k], i0 + (r + u + k) * di, a.drop, offset);
         }
       if constexpr (V == 4) {
-        if (a.drop.thresh && pairs && u < m) drop_apply_pair<V>(v[0], v[1], i + u * di, i + (u + 1) * di, a.drop, offset);   // (the second may be no pixel: not stored)
+        if (a.drop.thresh && pairs && u < m) drop_apply_pair<V>(v[0], v[1], i0 + (r + u) * di, i0 + (r + u + 1) * di, a.drop, offset);   // (the second may be no pixel: not stored)
       }
 #pragma unroll
       for (int k = 0; k < 2; ++k)
-        if (u + k < m) store_p<true, T, V>(y + (size_t)(p + (u + k) * a.rows) * a.ycs, v[k]);
+        if (u + k < m) store_nt<T, V>(y.ptr(r + u + k), v[k]);
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u) q[u] = next[u];
-    p = pn; m = mn;
-  }
+  });
 }
 
 // ---- backward ----
-// What a thread needs of its channels: xh = (x - mean) * rstd, z = xh * gamma + beta.
-template <int V> struct NormChan {
-  float mean[V], rstd[V], gamma[V], beta[V];
+// What a thread needs of its channels, with t = x - mean: z = t * scale + beta, scale = rstd * gamma.  (x - mean first: scale * x + const would
+// round twice at the size of mean * rstd.)  WHOLE: its V channels lie in one group, whose numbers it keeps once: 14 registers of 40 less
+// at V = 8.
+template <int V, bool WHOLE> struct NormChan {
+  static constexpr int W = WHOLE ? 1 : V;
+  float mean[W], rstd[W], scale[V], beta[V];
   __device__ __forceinline__ void load(const NormArgs& a, int img, int c0, bool on) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
+    for (int e = 0; e < W; ++e) {
       const size_t g = (size_t)img * a.groups + (on ? div_by(c0 + e, a.by_d) : 0);
       mean[e] = a.mean[g];
       rstd[e] = a.rstd[g];
-      gamma[e] = on && a.gamma ? a.gamma[c0 + e] : 1.f;
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      scale[e] = rstd[WHOLE ? 0 : e] * (on && a.gamma ? a.gamma[c0 + e] : 1.f);
       beta[e] = on && a.beta ? a.beta[c0 + e] : 0.f;
     }
   }
 };
-// v: x -> xh; g: dy (already dropped) -> dz
-template <int V> __device__ __forceinline__ void norm_dz(const NormArgs& a, const NormChan<V>& ch, float (&v)[V], float (&g)[V]) {
+// v: x -> t; g: dy (already dropped) -> dz
+template <int V, bool WHOLE> __device__ __forceinline__ void norm_dz(const NormArgs& a, const NormChan<V, WHOLE>& ch, float (&v)[V], float (&g)[V]) {
   float z[V];
 #pragma unroll
-  for (int e = 0; e < V; ++e) { v[e] = (v[e] - ch.mean[e]) * ch.rstd[e]; z[e] = v[e] * ch.gamma[e] + ch.beta[e]; }
+  for (int e = 0; e < V; ++e) { v[e] -= ch.mean[WHOLE ? 0 : e]; z[e] = v[e] * ch.scale[e] + ch.beta[e]; }
   act_grad_apply<V>(g, z, a.act);
 }
+// What takes dz and t to dx = rstd (gamma dz - S1 - xh S2) = scale dz - k1 - t k2, from (S1, S2) by group
+template <int V, bool WHOLE> struct NormBack {
+  static constexpr int W = WHOLE ? 1 : V;
+  float k1[W], k2[W];
+  __device__ __forceinline__ void set(int e, float2 s, float rstd) { k1[e] = rstd * s.x; k2[e] = rstd * rstd * s.y; }
+  __device__ __forceinline__ void apply(const NormChan<V, WHOLE>& ch, const float (&t)[V], float (&dz)[V]) const {
+#pragma unroll
+    for (int e = 0; e < V; ++e) dz[e] = (dz[e] * ch.scale[e] - k1[WHOLE ? 0 : e]) - t[e] * k2[WHOLE ? 0 : e];
+  }
+};
 // (A, B) of each of the workgroup's channels from its threads' sums, in sum[0 .. span), seen by every thread.  All threads call.
 // sum: TH * V numbers.
 template <int V, int TH> __device__ __forceinline__ void team_channels(const NormArgs& a, const NormTeam& t, float (&sa)[V], float (&sb)[V], float2* sum) {
@@ -625,78 +669,71 @@ template <int TH> __device__ __forceinline__ void team_group_sums(const NormArgs
 
 // The whole backward pass of a span in registers, x and dy read once: (A, B) of its channels go to ab[image][channel] for the parameters'
 // gradients over the images.
-template <typename T, int V, int R, int TH> __global__ __launch_bounds__(TH) void norm_team_grad_kernel(const NormArgs a) {
+template <typename T, int V, int R, int TH, bool WHOLE> __global__ __launch_bounds__(TH) void norm_team_grad_kernel(const NormArgs a) {
   __shared__ float2 sum[TH * V];
   __shared__ float2 tot[TH * V];
   const NormTeam t = span_team<V>(a);
-  const T* x = (const T*)a.x + (size_t)t.img * a.p * a.xcs + t.c0;
-  const T* dy = (const T*)a.dy + (size_t)t.img * a.p * a.dycs + t.c0;
+  const Walk<T, V> x(a, t, a.x, a.xcs, 0), dy(a, t, a.dy, a.dycs, 0), dx(a, t, a.y, a.ycs, 0);
+  const uint64_t i0 = ((uint64_t)t.img * a.p + t.row) * a.c + t.c0, di = (uint64_t)a.rows * a.c;
   Pack<T, V> q[R], g[R];
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int p = t.row + r * a.rows;
-    if (t.on && p < a.p) {
-      q[r] = *reinterpret_cast<const Pack<T, V>*>(x + (size_t)p * a.xcs);
-      g[r] = *reinterpret_cast<const Pack<T, V>*>(dy + (size_t)p * a.dycs);
+  for (int r = 0; r < R; ++r)
+    if (t.on && t.row + r * a.rows < a.p) {
+      q[r].load(x.ptr(r));
+      g[r].load(dy.ptr(r));
     }
-  }
-  NormChan<V> ch;
+  NormChan<V, WHOLE> ch;
   ch.load(a, t.img, t.c0, t.on);
   const uint64_t offset = a.drop.thresh ? drop_offset(a.drop) : 0;
   float sa[V], sb[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) sa[e] = sb[e] = 0.f;
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int p = t.row + r * a.rows;
-    if (t.on && p < a.p) {
+  for (int r = 0; r < R; ++r)
+    if (t.on && t.row + r * a.rows < a.p) {
       float v[V], w[V];
-      widen<T, V>(q[r], v);
-      widen<T, V>(g[r], w);
-      if (a.drop.thresh) drop_apply<V>(w, ((uint64_t)t.img * a.p + p) * a.c + t.c0, a.drop, offset);
-      norm_dz<V>(a, ch, v, w);
+      q[r].widen(v);
+      g[r].widen(w);
+      if (a.drop.thresh) drop_apply<V>(w, i0 + r * di, a.drop, offset);
+      norm_dz<V, WHOLE>(a, ch, v, w);
 #pragma unroll
       for (int e = 0; e < V; ++e) { sa[e] += w[e]; sb[e] += w[e] * v[e]; }
     }
-  }
+#pragma unroll
+  for (int e = 0; e < V; ++e) sb[e] *= ch.rstd[WHOLE ? 0 : e];
   team_channels<V, TH>(a, t, sa, sb, sum);
-  team_group_sums<TH>(a, t, sum, 1.f / ((float)a.p * (float)a.d), tot);
+  team_group_sums<TH>(a, t, sum, a.inv_m, tot);
   for (int c = threadIdx.x; c < a.span; c += TH) a.ab[(size_t)t.img * a.c + t.cbase + c] = sum[c];
   __syncthreads();
 #pragma unroll
-  for (int r = 0; r < R; ++r) { keep_packed<T, V>(q[r]); keep_packed<T, V>(g[r]); }
+  for (int r = 0; r < R; ++r) { q[r].keep(); g[r].keep(); }
   if (!t.on) return;
-  T* dx = (T*)a.y + (size_t)t.img * a.p * a.ycs + t.c0;
+  NormBack<V, WHOLE> back;
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int p = t.row + r * a.rows;
-    if (p < a.p) {
+  for (int e = 0; e < NormBack<V, WHOLE>::W; ++e) back.set(e, tot[div_by(t.col * V + e, a.by_d)], ch.rstd[e]);
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    if (t.row + r * a.rows < a.p) {
       float v[V], w[V];
-      widen<T, V>(q[r], v);
-      widen<T, V>(g[r], w);
-      if (a.drop.thresh) drop_apply<V>(w, ((uint64_t)t.img * a.p + p) * a.c + t.c0, a.drop, offset);
-      norm_dz<V>(a, ch, v, w);
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float2 s = tot[div_by(t.col * V + e, a.by_d)];
-        w[e] = ch.rstd[e] * (w[e] * ch.gamma[e] - s.x - v[e] * s.y);
-      }
-      store_v<T, V>(dx + (size_t)p * a.ycs, w);
+      q[r].widen(v);
+      g[r].widen(w);
+      if (a.drop.thresh) drop_apply<V>(w, i0 + r * di, a.drop, offset);
+      norm_dz<V, WHOLE>(a, ch, v, w);
+      back.apply(ch, v, w);
+      store_v<T, V>(dx.ptr(r), w);
     }
-  }
 }
 
-// dz (w) and xh (v) of the K pixels p, p + rows .. of the two-launch form from packed x and dy; K = 2 where a generator block is two
-// threads' work, m of them there
-template <typename T, int V> struct GradPixels {
+// dz (w) and t = x - mean (v) of K vectors of the two-launch form from packed x and dy, elements i and i + di on; K = 2 where a generator
+// block is two threads' work, m of them there
+template <typename T, int V, bool WHOLE> struct GradPixels {
   static constexpr int K = V == 4 ? 2 : 1;
   float v[K][V], w[K][V];
-  __device__ __forceinline__ void get(const NormArgs& a, const NormTeam& t, const NormChan<V>& ch, const Pack<T, V>* q, const Pack<T, V>* g, int p, int m,
+  __device__ __forceinline__ void get(const NormArgs& a, const NormChan<V, WHOLE>& ch, const Pack<T, V>* q, const Pack<T, V>* g, uint64_t i, uint64_t di, int m,
                                       uint64_t offset) {
-    const uint64_t i = ((uint64_t)t.img * a.p + p) * a.c + t.c0, di = (uint64_t)a.rows * a.c;
     bool pairs = false;
 #pragma unroll
-    for (int k = 0; k < K; ++k) { widen<T, V>(q[k], v[k]); widen<T, V>(g[k], w[k]); }
+    for (int k = 0; k < K; ++k) { q[k].widen(v[k]); g[k].widen(w[k]); }
     if constexpr (K == 2) {
       pairs = a.span % 8 == 0;
       if (a.drop.thresh && pairs) drop_apply_pair<V>(w[0], w[1], i, i + di, a.drop, offset);
@@ -705,52 +742,50 @@ template <typename T, int V> struct GradPixels {
     for (int k = 0; k < K; ++k)
       if (k < m) {
         if (a.drop.thresh && !pairs) drop_apply<V>(w[k], i + k * di, a.drop, offset);
-        norm_dz<V>(a, ch, v[k], w[k]);
+        norm_dz<V, WHOLE>(a, ch, v[k], w[k]);
       }
   }
 };
 
 // First launch: part[image][chunk][channel] = (A, B) of a chunk, and behind it s12[image][group][chunk] = (sum of gamma A, of gamma B) / (P D).
-template <typename T, int V, int TH, bool NT> __global__ __launch_bounds__(TH) void norm_chunk_sums_kernel(const NormArgs a) {
-  constexpr int U = sizeof(T) * V == 8 ? 4 : 2;
+template <typename T, int V, int U> struct GradBuffer { Pack<T, V> x[U], dy[U]; };
+template <typename T, int V, int TH, bool WHOLE> __global__ __launch_bounds__(TH) void norm_chunk_sums_kernel(const NormArgs a) {
+  constexpr int U = 2, K = GradPixels<T, V, WHOLE>::K;
+  typedef GradBuffer<T, V, U> B;
   __shared__ float2 sum[TH * V];
   __shared__ float2 tot[TH * V];
   int chunk, p0, p1;
   const NormTeam t = chunk_team<V>(a, blockIdx.x, a.chunks, a.ppc, chunk, p0, p1);
-  const T* x = (const T*)a.x + (size_t)t.img * a.p * a.xcs + t.c0;
-  const T* dy = (const T*)a.dy + (size_t)t.img * a.p * a.dycs + t.c0;
-  int p = p0 + t.row, m = batch_count(a, t, p, p1);
-  Pack<T, V> q[U], g[U], nq[U], ng[U];
-  load_batch<T, V, U, NT>(q, x, a.xcs, a.rows, p, m);
-  load_batch<T, V, U, NT>(g, dy, a.dycs, a.rows, p, m);
-  NormChan<V> ch;
+  const Walk<T, V> x(a, t, a.x, a.xcs, p0), dy(a, t, a.dy, a.dycs, p0);
+  Chunk<U, B> c(a, t, p1 - p0);
+  const auto load = [&](B& b, int r, int m) { x.load(b.x, r, m, a.nt); dy.load(b.dy, r, m, a.nt); };
+  if (t.on) c.fetch(c.b0, 0, load);
+  NormChan<V, WHOLE> ch;
   ch.load(a, t.img, t.c0, t.on);
   const uint64_t offset = a.drop.thresh ? drop_offset(a.drop) : 0;
+  const uint64_t i0 = ((uint64_t)t.img * a.p + p0 + t.row) * a.c + t.c0, di = (uint64_t)a.rows * a.c;
   float sa[V], sb[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) sa[e] = sb[e] = 0.f;
-  while (m) {
-    const int pn = p + U * a.rows, mn = batch_count(a, t, pn, p1);
-    load_batch<T, V, U, NT>(nq, x, a.xcs, a.rows, pn, mn);
-    load_batch<T, V, U, NT>(ng, dy, a.dycs, a.rows, pn, mn);
+  if (t.on)
+    c.finish(load, [&](B& b, int r, int m) {
 #pragma unroll
-    for (int u = 0; u < U; u += GradPixels<T, V>::K)
-      if (u < m) {
-        GradPixels<T, V> b;
-        b.get(a, t, ch, q + u, g + u, p + u * a.rows, m - u, offset);
+      for (int u = 0; u < U; u += K)
+        if (u < m) {
+          GradPixels<T, V, WHOLE> g;
+          g.get(a, ch, b.x + u, b.dy + u, i0 + (r + u) * di, di, m - u, offset);
 #pragma unroll
-        for (int k = 0; k < GradPixels<T, V>::K; ++k)
-          if (u + k < m) {
+          for (int k = 0; k < K; ++k)
+            if (u + k < m) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) { sa[e] += b.w[k][e]; sb[e] += b.w[k][e] * b.v[k][e]; }
-          }
-      }
+              for (int e = 0; e < V; ++e) { sa[e] += g.w[k][e]; sb[e] += g.w[k][e] * g.v[k][e]; }
+            }
+        }
+    });
 #pragma unroll
-    for (int u = 0; u < U; ++u) { q[u] = nq[u]; g[u] = ng[u]; }
-    p = pn; m = mn;
-  }
+  for (int e = 0; e < V; ++e) sb[e] *= ch.rstd[WHOLE ? 0 : e];
   team_channels<V, TH>(a, t, sa, sb, sum);
-  team_group_sums<TH>(a, t, sum, 1.f / ((float)a.p * (float)a.d), tot);
+  team_group_sums<TH>(a, t, sum, a.inv_m, tot);
   for (int c = threadIdx.x; c < a.span; c += TH) a.part[((size_t)t.img * a.chunks + chunk) * a.c + t.cbase + c] = sum[c];
   __syncthreads();
   for (int j = threadIdx.x; j < a.span / a.d; j += TH) a.s12[((size_t)t.img * a.groups + t.cbase / a.d + j) * a.chunks + chunk] = tot[j];
@@ -776,9 +811,10 @@ __device__ __forceinline__ void param_grads(const NormArgs& a, const float2* ab,
 __global__ __launch_bounds__(256) void norm_params_kernel(const NormArgs a, const float2* ab, int rows) { param_grads(a, ab, rows, blockIdx.x); }
 
 // Second launch: dx.  Its first `pblocks` workgroups sum the parameters' gradients instead.
-template <typename T, int V, int TH, bool NT> __global__ __launch_bounds__(TH) void norm_chunk_grad_kernel(const NormArgs a, int pblocks) {
+template <typename T, int V, int TH, bool WHOLE> __global__ __launch_bounds__(TH) void norm_chunk_grad_kernel(const NormArgs a, int pblocks) {
   static_assert(TH == 256, "param_grads");
-  constexpr int U = sizeof(T) * V == 8 ? 4 : 2;
+  constexpr int U = 2, K = GradPixels<T, V, WHOLE>::K;
+  typedef GradBuffer<T, V, U> B;
   __shared__ float2 tot[TH * V];
   if ((int)blockIdx.x < pblocks) {
     if (blockIdx.y == 0) param_grads(a, a.part, a.n * a.chunks, blockIdx.x);
@@ -786,13 +822,11 @@ template <typename T, int V, int TH, bool NT> __global__ __launch_bounds__(TH) v
   }
   int chunk, p0, p1;
   const NormTeam t = chunk_team<V>(a, blockIdx.x - pblocks, a.achunks, a.appc, chunk, p0, p1);
-  const T* x = (const T*)a.x + (size_t)t.img * a.p * a.xcs + t.c0;
-  const T* dy = (const T*)a.dy + (size_t)t.img * a.p * a.dycs + t.c0;
-  int p = p0 + t.row, m = batch_count(a, t, p, p1);
-  Pack<T, V> q[U], g[U], nq[U], ng[U];
-  load_batch<T, V, U, NT>(q, x, a.xcs, a.rows, p, m);
-  load_batch<T, V, U, NT>(g, dy, a.dycs, a.rows, p, m);
-  NormChan<V> ch;
+  const Walk<T, V> x(a, t, a.x, a.xcs, p0), dy(a, t, a.dy, a.dycs, p0), dx(a, t, a.y, a.ycs, p0);
+  Chunk<U, B> c(a, t, p1 - p0);
+  const auto load = [&](B& b, int r, int m) { x.load(b.x, r, m, a.nt); dy.load(b.dy, r, m, a.nt); };
+  if (t.on) c.fetch(c.b0, 0, load);
+  NormChan<V, WHOLE> ch;
   ch.load(a, t.img, t.c0, t.on);
   {
     const int lanes = 1 << a.jl, lane = threadIdx.x & (lanes - 1), groups = a.span / a.d;
@@ -810,32 +844,25 @@ template <typename T, int V, int TH, bool NT> __global__ __launch_bounds__(TH) v
     __syncthreads();
   }
   if (!t.on) return;
-  T* dx = (T*)a.y + (size_t)t.img * a.p * a.ycs + t.c0;
-  float s1[V], s2[V];
+  NormBack<V, WHOLE> back;
 #pragma unroll
-  for (int e = 0; e < V; ++e) { const float2 s = tot[div_by(t.col * V + e, a.by_d)]; s1[e] = s.x; s2[e] = s.y; }
+  for (int e = 0; e < NormBack<V, WHOLE>::W; ++e) back.set(e, tot[div_by(t.col * V + e, a.by_d)], ch.rstd[e]);
   const uint64_t offset = a.drop.thresh ? drop_offset(a.drop) : 0;
-  while (m) {
-    const int pn = p + U * a.rows, mn = batch_count(a, t, pn, p1);
-    load_batch<T, V, U, NT>(nq, x, a.xcs, a.rows, pn, mn);
-    load_batch<T, V, U, NT>(ng, dy, a.dycs, a.rows, pn, mn);
+  const uint64_t i0 = ((uint64_t)t.img * a.p + p0 + t.row) * a.c + t.c0, di = (uint64_t)a.rows * a.c;
+  c.finish(load, [&](B& b, int r, int m) {
 #pragma unroll
-    for (int u = 0; u < U; u += GradPixels<T, V>::K)
+    for (int u = 0; u < U; u += K)
       if (u < m) {
-        GradPixels<T, V> b;
-        b.get(a, t, ch, q + u, g + u, p + u * a.rows, m - u, offset);
+        GradPixels<T, V, WHOLE> g;
+        g.get(a, ch, b.x + u, b.dy + u, i0 + (r + u) * di, di, m - u, offset);
 #pragma unroll
-        for (int k = 0; k < GradPixels<T, V>::K; ++k)
+        for (int k = 0; k < K; ++k)
           if (u + k < m) {
-#pragma unroll
-            for (int e = 0; e < V; ++e) b.w[k][e] = ch.rstd[e] * (b.w[k][e] * ch.gamma[e] - s1[e] - b.v[k][e] * s2[e]);
-            store_p<true, T, V>(dx + (size_t)(p + (u + k) * a.rows) * a.ycs, b.w[k]);
+            back.apply(ch, g.v[k], g.w[k]);
+            store_nt<T, V>(dx.ptr(r + u + k), g.w[k]);
           }
       }
-#pragma unroll
-    for (int u = 0; u < U; ++u) { q[u] = nq[u]; g[u] = ng[u]; }
-    p = pn; m = mn;
-  }
+  });
 }
 
 // ---- any shape: workgroups of any channels, three launches (four backward).  What the forms above do not take: pixels of more vectors
@@ -870,7 +897,7 @@ template <typename T, int V> __global__ __launch_bounds__(256) void norm_stats_k
       Pack<T, V> q[U];
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (u < m) q[u] = load_p<false, T, V>(x + (size_t)(p + u * a.rows) * a.xcs);
+        if (u < m) q[u].load(x + (size_t)(p + u * a.rows) * a.xcs);
       stats_batch<T, V, U>(q, m, mean, m2, cnt);
     }
 #pragma unroll
@@ -930,10 +957,8 @@ __global__ __launch_bounds__(256) void norm_stats_join_kernel(const NormArgs a) 
 template <typename T, int V> __global__ __launch_bounds__(256) void norm_apply_kernel(const NormArgs a) {
   const NormTile t = NormTile::get<V>(a);
   if (!t.on) return;
-  NormChan<V> ch;
+  NormChan<V, false> ch;
   ch.load(a, t.img, t.c0, true);
-#pragma unroll
-  for (int e = 0; e < V; ++e) ch.rstd[e] *= ch.gamma[e];
   const uint64_t offset = a.drop.thresh ? drop_offset(a.drop) : 0;
   const T* x = (const T*)a.x + (size_t)t.img * a.p * a.xcs + t.c0;
   T* y = (T*)a.y + (size_t)t.img * a.p * a.ycs + t.c0;
@@ -941,7 +966,7 @@ template <typename T, int V> __global__ __launch_bounds__(256) void norm_apply_k
     float v[V];
     load_v<T, V>(x + (size_t)p * a.xcs, v);
 #pragma unroll
-    for (int e = 0; e < V; ++e) v[e] = (v[e] - ch.mean[e]) * ch.rstd[e] + ch.beta[e];
+    for (int e = 0; e < V; ++e) v[e] = (v[e] - ch.mean[e]) * ch.scale[e] + ch.beta[e];
     act_apply<V>(v, a.act);
     if (a.drop.thresh) drop_apply<V>(v, ((uint64_t)t.img * a.p + p) * a.c + t.c0, a.drop, offset);
     store_v<T, V>(y + (size_t)p * a.ycs, v);
@@ -953,7 +978,7 @@ template <typename T, int V> __global__ __launch_bounds__(256) void norm_bwd_sum
   __shared__ float2 red[256 * V];
   const NormTile t = NormTile::get<V>(a);
   if (t.on) {
-    NormChan<V> ch;
+    NormChan<V, false> ch;
     ch.load(a, t.img, t.c0, true);
     const uint64_t offset = a.drop.thresh ? drop_offset(a.drop) : 0;
     float sa[V], sb[V];
@@ -966,12 +991,12 @@ template <typename T, int V> __global__ __launch_bounds__(256) void norm_bwd_sum
       load_v<T, V>(x + (size_t)p * a.xcs, v);
       load_v<T, V>(dy + (size_t)p * a.dycs, g);
       if (a.drop.thresh) drop_apply<V>(g, ((uint64_t)t.img * a.p + p) * a.c + t.c0, a.drop, offset);
-      norm_dz<V>(a, ch, v, g);
+      norm_dz<V, false>(a, ch, v, g);
 #pragma unroll
       for (int e = 0; e < V; ++e) { sa[e] += g[e]; sb[e] += g[e] * v[e]; }
     }
 #pragma unroll
-    for (int e = 0; e < V; ++e) red[threadIdx.x * V + e] = make_float2(sa[e], sb[e]);
+    for (int e = 0; e < V; ++e) red[threadIdx.x * V + e] = make_float2(sa[e], sb[e] * ch.rstd[e]);
   }
   __syncthreads();
   const int nch = min(a.cb * V, a.c - (int)blockIdx.y * a.cb * V);
@@ -1017,11 +1042,11 @@ __global__ __launch_bounds__(256) void norm_bwd_join_kernel(const NormArgs a) {
 template <typename T, int V> __global__ __launch_bounds__(256) void norm_bwd_apply_kernel(const NormArgs a) {
   const NormTile t = NormTile::get<V>(a);
   if (!t.on) return;
-  NormChan<V> ch;
+  NormChan<V, false> ch;
   ch.load(a, t.img, t.c0, true);
-  float s1[V], s2[V];
+  NormBack<V, false> back;
 #pragma unroll
-  for (int e = 0; e < V; ++e) { const float2 s = a.s12[(size_t)t.img * a.groups + (t.c0 + e) / a.d]; s1[e] = s.x; s2[e] = s.y; }
+  for (int e = 0; e < V; ++e) back.set(e, a.s12[(size_t)t.img * a.groups + div_by(t.c0 + e, a.by_d)], ch.rstd[e]);
   const uint64_t offset = a.drop.thresh ? drop_offset(a.drop) : 0;
   const T* x = (const T*)a.x + (size_t)t.img * a.p * a.xcs + t.c0;
   const T* dy = (const T*)a.dy + (size_t)t.img * a.p * a.dycs + t.c0;
@@ -1031,9 +1056,8 @@ template <typename T, int V> __global__ __launch_bounds__(256) void norm_bwd_app
     load_v<T, V>(x + (size_t)p * a.xcs, v);
     load_v<T, V>(dy + (size_t)p * a.dycs, g);
     if (a.drop.thresh) drop_apply<V>(g, ((uint64_t)t.img * a.p + p) * a.c + t.c0, a.drop, offset);
-    norm_dz<V>(a, ch, v, g);
-#pragma unroll
-    for (int e = 0; e < V; ++e) g[e] = ch.rstd[e] * (g[e] * ch.gamma[e] - s1[e] - v[e] * s2[e]);
+    norm_dz<V, false>(a, ch, v, g);
+    back.apply(ch, v, g);
     store_v<T, V>(dx + (size_t)p * a.ycs, g);
   }
 }
