@@ -127,10 +127,14 @@ bool two_tiling(NormArgs& a, int v, int elem_bytes, bool backward) {
   while (k > 0 && (most % k || k * unit / v > 256)) --k;
   if (k == 0) return false;
   set_team(a, v, 256, k * unit);
-  // first launch: long-lived workgroups (their numbers have to be joined); second: some 48 KB each, four a CU at least
+  // First launch: two long-lived workgroups a CU, whose numbers have to be joined.  Second: six a CU; of tensors beyond 192 MB pieces of 24 KB, or
+  // eight times what a workgroup reads to join the first one's numbers.
   const size_t bytes = (size_t)a.n * a.p * a.c * elem_bytes * (backward ? 2 : 1);
-  chunks_for(a, env_int("NORM_SWG", backward && elem_bytes == 4 ? 1024 : 512), a.chunks, a.ppc);
-  chunks_for(a, env_int("NORM_AWG", (int)std::min<size_t>(std::max<size_t>(bytes / 49152, 1024), 16384)), a.achunks, a.appc);
+  chunks_for(a, env_int("NORM_SWG", 512), a.chunks, a.ppc);
+  a.join = a.chunks * (a.span / a.d) <= 2048;
+  size_t second = 1536;
+  if (bytes > (size_t)192 << 20) second = std::min<size_t>(bytes / std::max(24576, (backward || a.join) * a.chunks * (a.span / a.d) * 64), 32768);
+  chunks_for(a, env_int("NORM_AWG", (int)second), a.achunks, a.appc);
   return true;
 }
 template <typename T, int V, bool WHOLE> void launch_two_whole(const NormArgs& a, bool backward, hipStream_t st) {
@@ -143,19 +147,21 @@ template <typename T, int V, bool WHOLE> void launch_two_whole(const NormArgs& a
     hipLaunchKernelGGL((norm_chunk_grad_kernel<T, V, TH, WHOLE>), dim3(pblocks + a.n * a.achunks, ny), dim3(TH), 0, st, a, pblocks);
     return;
   }
-  const int join = a.chunks * (a.span / a.d) <= env_int("NORM_JOIN", 2048);
   hipLaunchKernelGGL((norm_chunk_stats_kernel<T, V, TH>), g1, dim3(TH), 0, st, a);
-  if (!join) {
+  if (!a.join) {
     NormArgs b = a;
     b.jl = 6;
     hipLaunchKernelGGL(norm_join_kernel, dim3(a.n * a.groups), dim3(64), 0, st, b);
   }
-  hipLaunchKernelGGL((norm_chunk_apply_kernel<T, V, TH, WHOLE>), dim3(a.n * a.achunks, ny), dim3(TH), 0, st, a, join);
+  hipLaunchKernelGGL((norm_chunk_apply_kernel<T, V, TH, WHOLE>), dim3(a.n * a.achunks, ny), dim3(TH), 0, st, a);
 }
 template <typename T, int V> bool launch_two(NormArgs a, bool backward, hipStream_t st) {
   if (!two_tiling(a, V, sizeof(T), backward)) return false;
   const size_t bytes = (size_t)a.n * a.p * a.c * sizeof(T) * (backward ? 2 : 1);
-  a.nt = bytes > (size_t)env_int("NORM_NT_MB", 128) << 20;
+  // Reads go past the caches where the 256 MB last-level cache could not keep them for the second launch (151 MB: 66 us against 69 with
+  // non-temporal reads; 830 MB: 408 against 430 without).  Writes always do: what takes this form is beyond the L2 caches or near it, and the
+  // last-level cache is read no faster than memory (7.3 against 7.5 TB/s).
+  a.nt = bytes > (size_t)env_int("NORM_NT_MB", 256) << 20;
   if (a.slots == 1) launch_two_whole<T, V, true>(a, backward, st);
   else launch_two_whole<T, V, V == 1>(a, backward, st);
   return true;
@@ -242,11 +248,20 @@ int norm_call(const char* who, NormArgs& a, bool backward, int n, int h, int w, 
   return 0;
 }
 
-template <typename T> void launch_dropout(const void* x, const void* res, void* y, size_t count, const DropArgs& d, hipStream_t st) {
-  const bool aligned = ((uintptr_t)x | (uintptr_t)res | (uintptr_t)y) % 16 == 0;
-  const dim3 grid(grid_for((count + 7) / 8));
-  if (aligned) hipLaunchKernelGGL((dropout_kernel<T, true>), grid, dim3(256), 0, st, (const T*)x, (const T*)res, (T*)y, count, d);
-  else hipLaunchKernelGGL((dropout_kernel<T, false>), grid, dim3(256), 0, st, (const T*)x, (const T*)res, (T*)y, count, d);
+template <typename T> int launch_dropout(const T* x, const T* res, T* y, size_t count, const DropArgs& d, hipStream_t st) {
+  if (((uintptr_t)x | (uintptr_t)res | (uintptr_t)y) % 16) {
+    hipLaunchKernelGGL(dropout_any_kernel<T>, dim3(grid_for((count + 7) / 8)), dim3(256), 0, st, x, res, y, count, d);
+    return 0;
+  }
+  const size_t per = (size_t)256 * (16 / sizeof(T)) * DROP_U, grid = (count + per - 1) / per, bytes = count * sizeof(T);
+  if (grid >= 1u << 24) return -1;
+  const dim3 g((unsigned)grid), b(256);
+  // all accesses past the caches beyond 160 MB of reads (202 MB: 64 us against 74 plain; 75 MB: 25.6 against 24.7); the writes alone where
+  // there is no residual and they pass the L2 caches (75 MB: 23.0 against 24.7; with a residual 38.4 against 35.4)
+  if (bytes * (res ? 2 : 1) > (size_t)160 << 20) hipLaunchKernelGGL((dropout_kernel<T, true, true>), g, b, 0, st, x, res, y, count, d);
+  else if (!res && bytes > (size_t)32 << 20) hipLaunchKernelGGL((dropout_kernel<T, false, true>), g, b, 0, st, x, res, y, count, d);
+  else hipLaunchKernelGGL((dropout_kernel<T, false, false>), g, b, 0, st, x, res, y, count, d);
+  return 0;
 }
 
 }  // namespace
@@ -291,9 +306,12 @@ int fisr_train_dropout(const void* x, const void* residual, void* y, size_t coun
   DeviceGuard guard(device_of(y));
   NORM_HIP_OK(guard.err);
   const hipStream_t st = (hipStream_t)stream;
-  if (type == FISR_TYPE_F32) launch_dropout<float>(x, residual, y, count, d, st);
-  else if (type == FISR_TYPE_F16) launch_dropout<f16_t>(x, residual, y, count, d, st);
-  else launch_dropout<b16_t>(x, residual, y, count, d, st);
+  const auto run = [&](auto* t) {
+    typedef std::remove_pointer_t<decltype(t)> T;
+    return launch_dropout<T>((const T*)x, (const T*)residual, (T*)y, count, d, st);
+  };
+  if ((type == FISR_TYPE_F32 ? run((float*)nullptr) : type == FISR_TYPE_F16 ? run((f16_t*)nullptr) : run((b16_t*)nullptr)) < 0)
+    return bad("more than 2^36 elements");
   NORM_HIP_OK(hipGetLastError());
   return 0;
 }

@@ -158,6 +158,8 @@ template <typename T, int V> __device__ __forceinline__ void store_nt(T* p, cons
   q.round(v);
   q.store_nt(p);
 }
+// Between a non-temporal access and a plain one of the same address in two branches: the compiler would make them one access and drop the hint.
+#define KEEP_APART(text) asm volatile("; " text)
 
 // ---- activations ----
 __device__ __forceinline__ float sigmoid_f(float z) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * z)); }
@@ -211,7 +213,7 @@ struct NormArgs {
   int n, p, c, groups, d;
   int cb, rows, span;                                  // columns and rows of a workgroup's threads, its channels
   int chunks, ppc;                                     // chunks of an image's pixels, pixels of a chunk: chunks = ceil(p / ppc)
-  int achunks, appc;                                   // ... in the second of two launches
+  int achunks, appc, join;                             // ... in the second of two launches; whether that joins the first one's numbers
   int slots, per_group, jl;                            // see team_sums
   uint32_t by_d, by_cb, by_rows, by_per_group;               // for div_by
   float eps, inv_m;                                    // inv_m: 1 / (p * d)
@@ -309,9 +311,11 @@ template <typename T, int V> struct Walk {
   __device__ __forceinline__ T* ptr(int r) const { return reinterpret_cast<T*>(base + (size_t)r * step + at); }
   template <int U> __device__ __forceinline__ void load(Pack<T, V> (&q)[U], int r, int m, int nt) const {      // nt: past the caches
     if (nt) {
+      KEEP_APART("past the caches");
 #pragma unroll
       for (int u = 0; u < U; ++u)
         if (u < m) q[u].load_nt(ptr(r + u));
+      KEEP_APART("end");
     } else {
 #pragma unroll
       for (int u = 0; u < U; ++u)
@@ -533,7 +537,7 @@ template <int V> __device__ __forceinline__ void drop_apply_pair(float (&v0)[V],
 }
 
 
-template <typename T, int V, int TH, bool WHOLE> __global__ __launch_bounds__(TH) void norm_chunk_apply_kernel(const NormArgs a, int join) {
+template <typename T, int V, int TH, bool WHOLE> __global__ __launch_bounds__(TH) void norm_chunk_apply_kernel(const NormArgs a) {
   constexpr int U = 4, W = WHOLE ? 1 : V;
   typedef Batch<T, V, U> B;
   __shared__ float mean_s[TH * V], rstd_s[TH * V];
@@ -551,7 +555,7 @@ template <typename T, int V, int TH, bool WHOLE> __global__ __launch_bounds__(TH
     scale[e] = t.on && a.gamma ? a.gamma[t.c0 + e] : 1.f;
     beta[e] = t.on && a.beta ? a.beta[t.c0 + e] : 0.f;
   }
-  if (join) {
+  if (a.join) {
     const int groups = div_by(a.span, a.by_d);
     join_groups<TH, 4>(a, g0, groups, mean_s, rstd_s);
     __syncthreads();
@@ -562,8 +566,8 @@ template <typename T, int V, int TH, bool WHOLE> __global__ __launch_bounds__(TH
 #pragma unroll
   for (int e = 0; e < V; ++e) {
     const int g = div_by(t.col * V + (WHOLE ? 0 : e), a.by_d);
-    if (e < W) mean[e] = join ? mean_s[g] : mg[g];
-    scale[e] *= join ? rstd_s[g] : rg[g];
+    if (e < W) mean[e] = a.join ? mean_s[g] : mg[g];
+    scale[e] *= a.join ? rstd_s[g] : rg[g];
   }
   const uint64_t offset = a.drop.thresh ? drop_offset(a.drop) : 0;
   const uint64_t i0 = ((uint64_t)t.img * a.p + p0 + t.row) * a.c + t.c0, di = (uint64_t)a.rows * a.c;
@@ -1062,28 +1066,71 @@ template <typename T, int V> __global__ __launch_bounds__(256) void norm_bwd_app
   }
 }
 
-// ---- dropout: y = drop(x) [+ res]; a thread per generator block of eight elements ----
-template <typename T, bool ALIGNED> __global__ __launch_bounds__(256) void dropout_kernel(const T* x, const T* res, T* y, size_t count, DropArgs d) {
+// ---- dropout: y = drop(x) [+ res] ----
+// A workgroup takes 256 x DROP_U vectors of 16 bytes that follow each other; float32: a generator block is two lanes' work, see
+// drop_apply_pair.  Bound by memory: 13 x 271 x 495 x 29 float32 without a residual in 65 us = 6.3 TB/s, 32 x 96 x 96 x 64 bfloat16 with one in
+// 18.2 us = 6.2 TB/s.  Two and four times as much work a workgroup: 67 and 69 us, 18.6 and 18.7 us.
+constexpr int DROP_U = 4;
+template <typename T, bool NT, bool NT_OUT> __global__ __launch_bounds__(256) void dropout_kernel(const T* x, const T* res, T* y, size_t count, DropArgs d) {
+  constexpr int V = 16 / sizeof(T), U = DROP_U;
+  const uint64_t offset = d.thresh ? drop_offset(d) : 0;
+  const size_t first = (size_t)blockIdx.x * (256 * U * V);
+  const T* const xb = x + first;                             // uniform: the threads' parts of the addresses have 32 bits
+  const T* const rb = res + first;
+  T* const yb = y + first;
+  const uint32_t at = threadIdx.x * V;
+  if (first + 256 * U * V > count) {                         // the last workgroup
+    for (uint32_t e = threadIdx.x; first + e < count; e += 256) {
+      float v[1] = {(float)xb[e]};
+      if (d.thresh) drop_apply<1>(v, first + e, d, offset);
+      yb[e] = (T)(res ? v[0] + (float)rb[e] : v[0]);
+    }
+    return;
+  }
+  Pack<T, V> q[U], r[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const T *xp = xb + u * 256 * V + at, *rp = rb + u * 256 * V + at;
+    if constexpr (NT) q[u].load_nt(xp);
+    else q[u].load(xp);
+    if (res) {
+      if constexpr (NT) r[u].load_nt(rp);
+      else r[u].load(rp);
+    }
+  }
+  float v[2][V];
+#pragma unroll
+  for (int u = 0; u < U; u += 2) {
+    q[u].widen(v[0]);
+    q[u + 1].widen(v[1]);
+    const uint64_t i = first + u * 256 * V + at;
+    if (d.thresh) {
+      if constexpr (V == 4) drop_apply_pair<V>(v[0], v[1], i, i + 256 * V, d, offset);
+      else { drop_apply<V>(v[0], i, d, offset); drop_apply<V>(v[1], i + 256 * V, d, offset); }
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (res) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[k][e] += r[u + k].get(e);
+      }
+      if constexpr (NT_OUT) store_nt<T, V>(yb + (u + k) * 256 * V + at, v[k]);
+      else store_v<T, V>(yb + (u + k) * 256 * V + at, v[k]);
+    }
+  }
+}
+// tensors that allow no vector accesses: a thread per generator block
+template <typename T> __global__ __launch_bounds__(256) void dropout_any_kernel(const T* x, const T* res, T* y, size_t count, DropArgs d) {
   const size_t blocks = (count + 7) / 8, stride = (size_t)gridDim.x * 256;
   const uint64_t offset = d.thresh ? drop_offset(d) : 0;
   for (size_t b = (size_t)blockIdx.x * 256 + threadIdx.x; b < blocks; b += stride) {
-    float v[8], r[8];
-    if (ALIGNED && 8 * b + 8 <= count) {
-      load_v<T, 8>(x + 8 * b, v);
-      if (res) load_v<T, 8>(res + 8 * b, r);
-      if (d.thresh) drop_apply<8>(v, 8 * b, d, offset);
-      if (res)
+    float v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] += r[e];
-      store_v<T, 8>(y + 8 * b, v);
-    } else {
+    for (int e = 0; e < 8; ++e) v[e] = 8 * b + e < count ? (float)x[8 * b + e] : 0.f;
+    if (d.thresh) drop_apply<8>(v, 8 * b, d, offset);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = 8 * b + e < count ? (float)x[8 * b + e] : 0.f;
-      if (d.thresh) drop_apply<8>(v, 8 * b, d, offset);
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (8 * b + e < count) y[8 * b + e] = (T)(res ? v[e] + (float)res[8 * b + e] : v[e]);
-    }
+    for (int e = 0; e < 8; ++e)
+      if (8 * b + e < count) y[8 * b + e] = (T)(res ? v[e] + (float)res[8 * b + e] : v[e]);
   }
 }
 
