@@ -25,12 +25,16 @@ int env_int(const char* name, int def) { const char* e = getenv(name); return e 
 constexpr int env_int(const char*, int def) { return def; }
 #endif
 
-// Chunks of an image's pixels for about `groups` workgroups in all, of at least 8192 elements each (32 a thread).
-void chunks_for(const NormArgs& a, int workgroups, int& chunks, int& ppc) {
+// Chunks of an image's pixels for about `workgroups` in all, of at least `least` elements each.
+void chunks_for(const NormArgs& a, int workgroups, int least, int& chunks, int& ppc) {
   const int want = std::max(1, workgroups / a.n);
-  ppc = std::max((a.p + want - 1) / want, (8191 + a.c) / a.c);
+  ppc = std::max((a.p + want - 1) / want, (least - 1 + a.c) / a.c);
   chunks = (a.p + ppc - 1) / ppc;
 }
+// Two vectors a thread, 1024 elements at the least: small tensors want many workgroups (5 x 67 x 45 x 36 float32 in 11.4 us at 2 vectors, 14.0 at 8;
+// 2 x 40 x 50 x 9 bfloat16 in 8.8 at 1024 elements, 14.0 at 8192)
+constexpr int LEAST_ELEMENTS = 1024;
+constexpr int least_chunk(int v) { return v * 512 > LEAST_ELEMENTS ? v * 512 : LEAST_ELEMENTS; }
 constexpr int MOST_CHUNK_GROUPS = 2048;                          // of a batch, by chunks_for: what the workspace is made for
 
 // Workspace: `part` of n * chunks * c float2, and for the backward pass s12 of n * groups * chunks and ab of n * c.  Not a function of the
@@ -38,7 +42,7 @@ constexpr int MOST_CHUNK_GROUPS = 2048;                          // of a batch, 
 struct WsLayout { size_t part, s12, ab; };
 WsLayout ws_layout(const NormArgs& a, bool backward) {
   int chunks, ppc;
-  chunks_for(a, MOST_CHUNK_GROUPS, chunks, ppc);
+  chunks_for(a, MOST_CHUNK_GROUPS, LEAST_ELEMENTS, chunks, ppc);
   WsLayout w{(size_t)a.n * chunks * a.c, 0, 0};
   if (backward) { w.s12 = (size_t)a.n * a.groups * chunks; w.ab = (size_t)a.n * a.c; }
   return w;
@@ -130,11 +134,11 @@ bool two_tiling(NormArgs& a, int v, int elem_bytes, bool backward) {
   // First launch: two long-lived workgroups a CU, whose numbers have to be joined.  Second: six a CU; of tensors beyond 192 MB pieces of 24 KB, or
   // eight times what a workgroup reads to join the first one's numbers.
   const size_t bytes = (size_t)a.n * a.p * a.c * elem_bytes * (backward ? 2 : 1);
-  chunks_for(a, env_int("NORM_SWG", 512), a.chunks, a.ppc);
+  chunks_for(a, env_int("NORM_SWG", 512), least_chunk(v), a.chunks, a.ppc);
   a.join = a.chunks * (a.span / a.d) <= 2048;
   size_t second = 1536;
   if (bytes > (size_t)192 << 20) second = std::min<size_t>(bytes / std::max(24576, (backward || a.join) * a.chunks * (a.span / a.d) * 64), 32768);
-  chunks_for(a, env_int("NORM_AWG", (int)second), a.achunks, a.appc);
+  chunks_for(a, env_int("NORM_AWG", (int)second), least_chunk(v), a.achunks, a.appc);
   return true;
 }
 template <typename T, int V, bool WHOLE> void launch_two_whole(const NormArgs& a, bool backward, hipStream_t st) {
@@ -169,7 +173,7 @@ template <typename T, int V> bool launch_two(NormArgs a, bool backward, hipStrea
 
 // Any shape.
 template <typename T, int V> void launch_any(NormArgs a, bool backward, hipStream_t st) {
-  chunks_for(a, MOST_CHUNK_GROUPS, a.chunks, a.ppc);
+  chunks_for(a, MOST_CHUNK_GROUPS, 8192, a.chunks, a.ppc);
   const int cv = (a.c + V - 1) / V, ny = (cv + 255) / 256;
   a.cb = (cv + ny - 1) / ny;
   a.rows = 256 / a.cb;
