@@ -87,6 +87,9 @@ def parse_args(argv=None):
     p.add_argument("--tmm_lambda", type=float, default=1.0)
     p.add_argument("--td_lambda", type=float, default=0.1)
     p.add_argument("--ss2_lambda", type=float, default=1.0)
+    p.add_argument("--dropout", type=float, default=0.0, metavar="P",
+                   help="--phase train: dropout of probability P between the two convs of every residual block (the reference has none); "
+                        "off in validation, and the checkpoints are the same variables")
     p.add_argument("--save_tf_bundle", action="store_true",
                    help="--phase train: also write every checkpoint as a TensorFlow checkpoint-V2 bundle (FISRnet-<step>.index/.data-*)")
     p.add_argument("--synthetic_train", type=int, default=0, metavar="N",

@@ -43,14 +43,21 @@ class _Conv:
 
 
 class TrainNet:
-    def __init__(self, weights=None, device="cuda:0", seed=2020, lambdas=None):
+    def __init__(self, weights=None, device="cuda:0", seed=2020, lambdas=None, dropout=0.0, dropout_seed=2020):
+        """dropout: probability of a dropout between the two convs of every residual block while `training` is set (the reference has
+        none: 0); its masks are a function of dropout_seed, the step and the block, so a run repeats and resumes with the same ones, and
+        every rank of a data-parallel run takes a seed of its own."""
         import torch
+        if not 0.0 <= dropout < 1.0:
+            raise ValueError(f"dropout = {dropout} is not in [0, 1)")
         self.torch = torch
         self.L = _lib.lib()
         self.device = torch.device(device)
         if self.device.type != "cuda":
             raise _lib.FisrError("fisr_amd.train needs a GPU device (there is no CPU fallback)")
         self.lam = dict(LAMBDAS if lambdas is None else lambdas)
+        self.training = True
+        self.dropout_p, self.dropout_seed, self._dropouts = float(dropout), int(dropout_seed), 0
         W = weights if weights is not None else _weights.synthetic_weights(seed)
         _weights.check_complete(W)
         self.convs = OrderedDict()
@@ -208,6 +215,27 @@ class TrainNet:
         self.tape.append(("up", x, y))
         return y
 
+    def next_dropout(self, p):
+        """The next norm.Dropout of this step: (dropout_seed; step and number within it)."""
+        from . import norm
+        self._dropouts += 1
+        return norm.Dropout(p, self.dropout_seed, (self.step_count << 20) + self._dropouts)
+
+    def dropout(self, x, drop, residual=None):
+        """norm.dropout, recorded: drop(x) [+ residual]."""
+        from . import norm
+        y = norm.dropout(x, drop, residual=residual)
+        self.tape.append(("dropout", x, residual, y, drop))
+        return y
+
+    def group_norm(self, x, groups, gamma, beta, ggamma, gbeta, eps=1e-5, act="none", drop=None):
+        """norm.group_norm, recorded: drop(act(gn(x) * gamma + beta)); backward() adds the parameters' gradients to ggamma and gbeta, as
+        the convs' do (four passes share the weights)."""
+        from . import norm
+        y, stats = norm.group_norm(x, groups, gamma, beta, eps=eps, act=act, dropout=drop)
+        self.tape.append(("norm", x, stats, groups, gamma, beta, ggamma, gbeta, act, drop, y))
+        return y
+
     def level_input(self, x29, prev_pred):
         """FISRnet.py:84,113-116,144-147: the level's input, channels padded to a multiple of 16 with zeros."""
         n, h, w, _ = x29.shape
@@ -223,6 +251,8 @@ class TrainNet:
     # ------------------------------------------------------------------ the network (FISRnet.py:73-173, ops.py:39-76)
     def _res_block(self, x, p, relu_after=False):
         a = self.conv(p + "/conv/0", x, flags=RELU_IN | RELU_OUT)
+        if self.training and self.dropout_p:
+            a = self.dropout(a, self.next_dropout(self.dropout_p))
         return self.conv(p + "/conv/1", a, res=x, flags=RELU_OUT if relu_after else 0)
 
     def _enc(self, x, p):
@@ -353,6 +383,24 @@ class TrainNet:
                     if flags & RELU_IN:
                         self._ck(L.fisr_train_relu_bwd(self._p(ds), self._p(xs), self._p(ds), ds.numel(), self._st()))
                     self._acc(grads, xs, ds)
+            elif kind == "dropout":
+                from . import norm
+                _, x, residual, y, drop = ent
+                g = grads.pop(y.data_ptr(), None)
+                if g is None:
+                    continue
+                self._acc(grads, x, norm.dropout_backward(g, drop))
+                if residual is not None:
+                    self._acc(grads, residual, g)
+            elif kind == "norm":
+                from . import norm
+                _, x, stats, groups, gamma, beta, ggamma, gbeta, act, drop, y = ent
+                g = grads.pop(y.data_ptr(), None)
+                if g is None:
+                    continue
+                dx, _, _ = norm.group_norm_backward(g, x, stats, groups, gamma, beta, act=act, dropout=drop, dgamma=ggamma, dbeta=gbeta,
+                                                    accumulate=True)
+                self._acc(grads, x, dx)
             elif kind == "pool":
                 _, x, y = ent
                 g = grads.pop(y.data_ptr(), None)
@@ -406,6 +454,7 @@ class TrainNet:
         gradients are left accumulated in the conv states (call zero_grad() first)."""
         torch, L = self.torch, self.L
         self.tape = []
+        self._dropouts = 0
         # The four passes share the weights, so they run as ONE pass over a batch of 4B: windows 0, 1, 2 (stride 1,
         # FISRnet.py:283-310) and the stride-2 window (:403-409) stacked along the batch axis -- a quarter of the kernel
         # launches, four times the work per launch, the same numbers (every sample is convolved independently).

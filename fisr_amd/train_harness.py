@@ -134,7 +134,7 @@ def run_train(args):
         counter = 0
         print(" [!] Load failed...")
     lam = dict(recn=args.recn_lambda, tm1=args.tm1_lambda, tm2=args.tm2_lambda, tmm=args.tmm_lambda, td=args.td_lambda, ss2=args.ss2_lambda)
-    net = ft.TrainNet(W, device=dev, lambdas=lam)
+    net = ft.TrainNet(W, device=dev, lambdas=lam, dropout=getattr(args, "dropout", 0.0), dropout_seed=args.exp_num * 65536 + rank)
     if opt_state is not None:
         net.load_optimizer_state(opt_state, fallback_step=counter)   # Adam moments + the step of the bias correction (saver.restore, FISRnet.py:1108)
     else:
@@ -195,6 +195,7 @@ def run_train(args):
                   % ((epoch, lr, (time.time() - start_time) / 60) + tuple(m)))
         # validation (FISRnet.py:713-742): stride-1 windows only, reconstruction loss and PSNR of the overlapped sequence
         vl, vp = [], []
+        net.training = False
         for vi in range(val_iter):
             sl = slice(args.val_batch_size * vi, args.val_batch_size * (vi + 1))
             vb = ft.to_device_batch({a: va[b][sl] for a, b in keymap}, dev)
@@ -206,6 +207,7 @@ def run_train(args):
             gt = vb["label21"].reshape(b_, h_, w_, 7, 3).permute(0, 3, 1, 2, 4)
             vl.append(float(((ov - gt) ** 2).mean()))
             vp.append(_psnr(ov, vb["label21"]))
+        net.training = True
         if vl:
             print("######### Validation (average),Epoch: [%4d/%4d]-th epoch, time: %4.2f(min.), val_PSNR: %.3f[dB], "
                   "recnLoss: %.6f #########" % (epoch, args.epoch, (time.time() - start_time) / 60, np.mean(vp), np.mean(vl)))
