@@ -129,7 +129,8 @@ bool two_tiling(NormArgs& a, int v, int elem_bytes, bool backward) {
   const int unit = span_unit(a, v), most = a.c / unit;
   int k = most;
   while (k > 0 && (most % k || k * unit / v > 256)) --k;
-  if (k == 0) return false;
+  // (no such span, or one of few columns with more channels beside it: workgroups of any channels read whole lines)
+  if (k == 0 || (k < most && k * unit / v < 64)) return false;
   set_team(a, v, 256, k * unit);
   // First launch: two long-lived workgroups a CU, whose numbers have to be joined.  Second: six a CU; of tensors beyond 192 MB pieces of 24 KB, or
   // eight times what a workgroup reads to join the first one's numbers.
@@ -242,7 +243,10 @@ int norm_call(const char* who, NormArgs& a, bool backward, int n, int h, int w, 
   a.part = (float2*)ws;
   a.s12 = a.part + lay.part;
   a.ab = a.s12 + lay.s12;
-  DeviceGuard guard(device_of(a.y));
+  const int dev = device_of(a.y);
+  if (dev < 0 || device_of(a.x) != dev || (backward && device_of(a.dy) != dev) || (ws && device_of(ws) != dev) || device_of(mean_rstd) != dev)
+    return bad("a pointer is not to memory of the output's device");
+  DeviceGuard guard(dev);
   NORM_HIP_OK(guard.err);
   const hipStream_t st = (hipStream_t)stream;
   if (type == FISR_TYPE_F32) launch<float>(a, backward, st);
@@ -307,7 +311,9 @@ int fisr_train_dropout(const void* x, const void* residual, void* y, size_t coun
   if (count == 0) return 0;
   if (!x || !y) return bad("null tensor");
   if (((uintptr_t)x | (uintptr_t)residual | (uintptr_t)y) % es) return bad("a pointer is not aligned to its element");
-  DeviceGuard guard(device_of(y));
+  const int dev = device_of(y);
+  if (dev < 0 || device_of(x) != dev || (residual && device_of(residual) != dev)) return bad("a pointer is not to memory of the output's device");
+  DeviceGuard guard(dev);
   NORM_HIP_OK(guard.err);
   const hipStream_t st = (hipStream_t)stream;
   const auto run = [&](auto* t) {

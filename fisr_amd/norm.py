@@ -125,6 +125,16 @@ def _drop(dropout, dev):
 _stream = torch._C._cuda_getCurrentRawStream          # of a device's index: torch.cuda.current_stream(...).cuda_stream without the object
 
 
+def _apart(out, out_cs, t, t_cs, what):
+    """An output may be the tensor itself or lie beside it, in other channels of the same pixels too, but not across it."""
+    a, b, size = out.data_ptr(), t.data_ptr(), t.element_size()
+    c, pixels = t.shape[-1], t.numel() // t.shape[-1]
+    if (a == b and out_cs == t_cs) or a >= b + ((pixels - 1) * t_cs + c) * size or b >= a + ((pixels - 1) * out_cs + c) * size:
+        return
+    if out_cs != t_cs or not c * size <= (a - b) % (t_cs * size) <= (t_cs - c) * size:
+        raise ValueError(f"{what} overlaps an input that it is not")
+
+
 def _out(x, out, cs, dev, what):
     """The output tensor and its pixel stride."""
     if out is not None:
@@ -146,6 +156,8 @@ def group_norm(x, groups, gamma=None, beta=None, *, eps=1e-5, act="none", dropou
     code, dev = _type(x)
     x_cs = _pixel_stride(x, "x")
     y, y_cs = _out(x, out, x_cs, dev, "out")
+    if out is not None and x.numel():
+        _apart(y, y_cs, x, x_cs, "out")
     stats = x.new_empty((2, n, max(groups, 0)), dtype=torch.float32)
     g, b, a, d, st = _param(gamma, dev, (c,), "gamma"), _param(beta, dev, (c,), "beta"), _act(act), _drop(dropout, dev), _stream(dev)
     rc = _fn.gn(x.data_ptr(), x_cs, g, b, y.data_ptr(), y_cs, stats.data_ptr(), n, h, w, c, groups, eps, a, d, code, None, 0, st)
@@ -161,12 +173,16 @@ def group_norm_backward(dy, x, stats, groups, gamma=None, beta=None, *, act="non
                         accumulate=False):
     """Gradients of group_norm: (dx, dgamma, dbeta) from dy, the forward pass' x and stats and the same parameters, activation and
     dropout.  dgamma and dbeta (float32 [C]) are made where they are not given; given ones are overwritten or, with `accumulate`, added
-    to.  `dx` may be dy."""
+    to.  `dx` may be dy, or x."""
     n, h, w, c = _images(x, groups)
     code, dev = _type(x)
     _like(dy, x, dev, "dy")
-    x_cs = _pixel_stride(x, "x")
+    x_cs, dy_cs = _pixel_stride(x, "x"), _pixel_stride(dy, "dy")
+    given = dx is not None and x.numel() > 0
     dx, dx_cs = _out(x, dx, x_cs, dev, "dx")
+    if given:
+        _apart(dx, dx_cs, dy, dy_cs, "dx")
+        _apart(dx, dx_cs, x, x_cs, "dx")
     if accumulate and (dgamma is None or dbeta is None):
         raise ValueError("accumulate: dgamma and dbeta have to be given")
     if dgamma is None:
@@ -174,7 +190,7 @@ def group_norm_backward(dy, x, stats, groups, gamma=None, beta=None, *, act="non
     if dbeta is None:
         dbeta = x.new_empty(c, dtype=torch.float32)
     ws, nbytes = _workspace(x, n, h, w, c, groups, 1)
-    rc = _fn.gn_bwd(x.data_ptr(), x_cs, dy.data_ptr(), _pixel_stride(dy, "dy"), _param(gamma, dev, (c,), "gamma"), _param(beta, dev, (c,), "beta"),
+    rc = _fn.gn_bwd(x.data_ptr(), x_cs, dy.data_ptr(), dy_cs, _param(gamma, dev, (c,), "gamma"), _param(beta, dev, (c,), "beta"),
                     _param(stats, dev, (2, n, groups), "stats"), dx.data_ptr(), dx_cs, _param(dgamma, dev, (c,), "dgamma"),
                     _param(dbeta, dev, (c,), "dbeta"), 1 if accumulate else 0, n, h, w, c, groups, _act(act), _drop(dropout, dev), code,
                     ws.data_ptr(), nbytes, _stream(dev))
@@ -190,6 +206,10 @@ def dropout(x, drop, residual=None, out=None):
     if not (x.is_contiguous() and (out is None or out.is_contiguous()) and (residual is None or residual.is_contiguous())):
         raise ValueError("dropout: dense tensors are wanted (the mask goes by an element's place in one)")
     res = _like(residual, x, dev, "residual").data_ptr() if residual is not None else None
+    if out is not None and x.numel():
+        _apart(y.view(-1), x.numel(), x.view(-1), x.numel(), "out")
+        if residual is not None:
+            _apart(y.view(-1), x.numel(), residual.view(-1), x.numel(), "out")
     rc = _fn.drop(x.data_ptr(), res, y.data_ptr(), x.numel(), _drop(drop, dev), code, _stream(dev))
     if rc < 0:
         _lib.check(rc)

@@ -404,7 +404,7 @@ FISR_API size_t fisr_train_groupnorm_workspace_bytes(int n, int h, int w, int c,
 FISR_API int fisr_train_groupnorm(const void* x, int x_cs, const float* gamma, const float* beta, void* y, int y_cs, float* mean_rstd, int n,
                      int h, int w, int c, int groups, float eps, int act, const fisr_dropout* drop, int type, void* workspace,
                      size_t workspace_bytes, void* stream);
-/* its gradients from the forward pass' x and mean_rstd: dx (may be dy, not x), and dgamma, dbeta [c] (nullable), overwritten or, with
+/* its gradients from the forward pass' x and mean_rstd: dx (may be dy or x), and dgamma, dbeta [c] (nullable), overwritten or, with
  * accumulate != 0, added to */
 FISR_API int fisr_train_groupnorm_bwd(const void* x, int x_cs, const void* dy, int dy_cs, const float* gamma, const float* beta,
                      const float* mean_rstd, void* dx, int dx_cs, float* dgamma, float* dbeta, int accumulate, int n, int h, int w, int c,

@@ -79,7 +79,8 @@ SHAPES = [
     (1, 1, 1, 1, 1), (1, 1, 1, 8, 1), (2, 1, 1, 64, 8), (3, 1, 2, 2, 2), (1, 1, 7, 6, 3), (2, 3, 3, 512, 32), (4, 6, 6, 256, 32), (1, 5, 9, 29, 29),
     (2, 13, 11, 29, 1), (2, 17, 9, 36, 4), (1, 24, 24, 64, 64), (3, 12, 12, 512, 1), (2, 19, 23, 40, 5), (2, 9, 7, 12, 2), (1, 3, 2, 600, 4),
     (1, 2, 3, 4104, 8), (2, 2, 2, 2060, 4), (1, 1, 3, 1027, 13), (37, 3, 5, 16, 16), (2, 96, 96, 64, 8), (1, 130, 70, 8, 2), (1, 191, 67, 3, 1),
-    (5, 31, 33, 24, 8), (300, 2, 2, 8, 4),
+    (5, 31, 33, 24, 8), (300, 2, 2, 8, 4), (2, 40, 30, 521, 521), (1, 96, 40, 1042, 521), (3, 70, 60, 1027, 13), (2, 60, 50, 2056, 4), (1, 210, 200, 72, 8),
+    (2, 130, 150, 96, 32),
 ]
 KINDS = [("f32", "none", 0.0), ("f32", "silu", 0.25), ("f16", "gelu", 0.0), ("f16", "relu", 0.1), ("bf16", "silu", 0.0), ("bf16", "gelu", 0.5), ("f32", "relu", 0.0),
          ("f32", "gelu", 0.1)]
@@ -175,9 +176,10 @@ def test_channel_ranges_of_wider_buffers(env, t, c, lo, hi):
     assert (dxo[..., :lo] == 7).all() and (dxo[..., hi:] == 7).all()
 
 
-def test_in_place(env):
+@pytest.mark.parametrize("shape", [(3, 33, 31, 32), (1, 90, 80, 64)])           # one launch, two
+def test_in_place(env, shape):
     torch, norm = env
-    x, dy, gamma, beta = _inputs(torch, 3, 33, 31, 32, "bf16", 11)
+    x, dy, gamma, beta = _inputs(torch, *shape, "bf16", 11)
     y, st = norm.group_norm(x, 4, gamma, beta, act="silu")
     dx, _, _ = norm.group_norm_backward(dy, x, st, 4, gamma, beta, act="silu")
     xi, di = x.clone(), dy.clone()
@@ -185,6 +187,9 @@ def test_in_place(env):
     assert yi.data_ptr() == xi.data_ptr() and torch.equal(yi, y) and torch.equal(sti, st)
     norm.group_norm_backward(di, x, st, 4, gamma, beta, act="silu", dx=di)
     assert torch.equal(di, dx)
+    xx = x.clone()
+    norm.group_norm_backward(dy, xx, st, 4, gamma, beta, act="silu", dx=xx)
+    assert torch.equal(xx, dx)
 
 
 @pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu"])

@@ -107,6 +107,34 @@ def test_dropout_refuses():
         assert f(*a, None) == -1
 
 
+def test_pointers_that_are_no_device_memory_are_refused():
+    """Whole calls with pointers to nothing, and to host memory: refused before a launch."""
+    host = ctypes.create_string_buffer(1 << 16)
+    for p in (P, ctypes.addressof(host) // 64 * 64 + 64):
+        assert _gn(x=p, y=p, st=p, ws=p) == -1 and b"memory" in lib.lib().fisr_last_error(None)
+        assert _gb(x=p, dy=p, dx=p, st=p, ws=p) == -1 and b"memory" in lib.lib().fisr_last_error(None)
+        assert lib.lib().fisr_train_dropout(p, None, p, 8, _drop(0.5), 0, None) == -1
+
+
+def test_outputs_across_an_input_are_refused():
+    import torch
+    from fisr_amd import norm
+    b = torch.zeros(2, 3, 4, 24)
+    cs = lambda t: norm._pixel_stride(t, "t")  # noqa: E731
+    far = torch.zeros(2, 3, 4, 8)
+    x = b[..., 4:12]
+    for ok in (x, b[..., 12:20], b[..., :4][..., :4], far):
+        if ok.shape == x.shape:
+            norm._apart(ok, cs(ok), x, cs(x), "out")
+    for bad in (b[..., 8:16], b[..., 0:8], b[..., 3:11], b.view(-1)[8:8 + far.numel()].view(far.shape)):
+        with pytest.raises(ValueError, match="overlaps"):
+            norm._apart(bad, cs(bad), x, cs(x), "out")
+    flat = torch.zeros(100)
+    with pytest.raises(ValueError, match="overlaps"):
+        norm._apart(flat[1:51], 50, flat[:50], 50, "out")
+    norm._apart(flat[50:], 50, flat[:50], 50, "out")
+
+
 def test_python_entries_refuse():
     import torch
     from fisr_amd import norm
