@@ -283,6 +283,36 @@ template <int V, int TH, typename F> __device__ __forceinline__ void team_sums(c
   __syncthreads();
 }
 
+// Two pixels' dropout of a thread with four channels: a generator block is eight, so lanes 2k and 2k + 1 want the same two blocks.  Each
+// computes one and they exchange halves.  The span's channels are a multiple of 8, so both lanes are at the same pixels.
+template <int V> __device__ __forceinline__ void drop_apply_pair(float (&v0)[V], float (&v1)[V], uint64_t i0, uint64_t i1, const DropArgs& d, uint64_t offset) {
+  static_assert(V == 4, "");
+  const bool odd = threadIdx.x & 1;
+  const Philox r = philox7((odd ? i1 : i0) >> 3, offset, d.seed);
+  const uint32_t s0 = odd ? r.w[0] : r.w[2], s1 = odd ? r.w[1] : r.w[3];
+  const uint32_t g0 = __builtin_amdgcn_mov_dpp(s0, 0xB1, 0xf, 0xf, true), g1 = __builtin_amdgcn_mov_dpp(s1, 0xB1, 0xf, 0xf, true);   // quad_perm 1, 0, 3, 2
+  const uint32_t a0 = odd ? g0 : r.w[0], a1 = odd ? g1 : r.w[1], b0 = odd ? r.w[2] : g0, b1 = odd ? r.w[3] : g1;
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    const uint32_t wa = e & 2 ? a1 : a0, wb = e & 2 ? b1 : b0;
+    v0[e] = (e & 1 ? wa >> 16 : wa & 0xffffu) >= d.thresh ? v0[e] * d.scale : 0.f;
+    v1[e] = (e & 1 ? wb >> 16 : wb & 0xffffu) >= d.thresh ? v1[e] * d.scale : 0.f;
+  }
+}
+
+
+// Dropout of the K = 1 or 2 vectors v of a thread, elements i and i + di on.  pairs: drop_apply_pair may be used.
+template <int V> __device__ __forceinline__ void drop_two(float (&v0)[V], float (&v1)[V], int k, bool pairs, uint64_t i, uint64_t di, const DropArgs& d, uint64_t offset) {
+  if constexpr (V == 4) {
+    if (pairs) {
+      drop_apply_pair<V>(v0, v1, i, i + di, d, offset);      // (the second may be no pixel: nobody uses it)
+      return;
+    }
+  }
+  drop_apply<V>(v0, i, d, offset);
+  if (k > 1) drop_apply<V>(v1, i + di, d, offset);
+}
+
 // ---- one launch, one read: a workgroup holds `span` channels (whole groups) of all pixels of an image in registers ----
 // Thread (row, col) keeps the vectors of column col at the pixels row + r * rows, r < R, as they were loaded (16-bit tensors packed).
 // What a second pass over memory would be is a pass over registers, so the mean comes first and the squares are about it.
@@ -372,15 +402,23 @@ template <typename T, int V, int R, int TH> __global__ __launch_bounds__(TH) voi
   for (int e = 0; e < V; ++e) gamma[e] *= tot[1][div_by(t.col * V + e, a.by_d)];
   const uint64_t offset = a.drop.thresh ? drop_offset(a.drop) : 0;
   const uint64_t i0 = ((uint64_t)t.img * a.p + t.row) * a.c + t.c0, di = (uint64_t)a.rows * a.c;
+  const bool pairs = V == 4 && a.span % 8 == 0;
 #pragma unroll
-  for (int r = 0; r < R; ++r)
+  for (int r = 0; r < R; r += 2)
     if (t.row + r * a.rows < a.p) {
-      float v[V];
+      float v[2][V];
+      const int m = r + 1 < R && t.row + (r + 1) * a.rows < a.p ? 2 : 1;
 #pragma unroll
-      for (int e = 0; e < V; ++e) v[e] = (q[r].get(e) - mean[e]) * gamma[e] + beta[e];
-      act_apply<V>(v, a.act);
-      if (a.drop.thresh) drop_apply<V>(v, i0 + r * di, a.drop, offset);
-      store_v<T, V>(y.ptr(r), v);
+      for (int k = 0; k < 2; ++k)
+        if (r + k < R && k < m) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) v[k][e] = (q[r + k < R ? r + k : r].get(e) - mean[e]) * gamma[e] + beta[e];
+          act_apply<V>(v[k], a.act);
+        }
+      if (a.drop.thresh) drop_two<V>(v[0], v[1], m, pairs, i0 + r * di, di, a.drop, offset);
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        if (r + k < R && k < m) store_v<T, V>(y.ptr(r + k), v[k]);
     }
 }
 
@@ -519,24 +557,6 @@ __global__ __launch_bounds__(64) void norm_join_kernel(const NormArgs a) {
   join_groups<64, 16>(a, blockIdx.x, 1, a.mean + blockIdx.x, a.rstd + blockIdx.x);
 }
 
-// Two pixels' dropout of a thread with four channels: a generator block is eight, so lanes 2k and 2k + 1 want the same two blocks.  Each
-// computes one and they exchange halves.  The span's channels are a multiple of 8, so both lanes are at the same pixels.
-template <int V> __device__ __forceinline__ void drop_apply_pair(float (&v0)[V], float (&v1)[V], uint64_t i0, uint64_t i1, const DropArgs& d, uint64_t offset) {
-  static_assert(V == 4, "");
-  const bool odd = threadIdx.x & 1;
-  const Philox r = philox7((odd ? i1 : i0) >> 3, offset, d.seed);
-  const uint32_t s0 = odd ? r.w[0] : r.w[2], s1 = odd ? r.w[1] : r.w[3];
-  const uint32_t g0 = __builtin_amdgcn_mov_dpp(s0, 0xB1, 0xf, 0xf, true), g1 = __builtin_amdgcn_mov_dpp(s1, 0xB1, 0xf, 0xf, true);   // quad_perm 1, 0, 3, 2
-  const uint32_t a0 = odd ? g0 : r.w[0], a1 = odd ? g1 : r.w[1], b0 = odd ? r.w[2] : g0, b1 = odd ? r.w[3] : g1;
-#pragma unroll
-  for (int e = 0; e < V; ++e) {
-    const uint32_t wa = e & 2 ? a1 : a0, wb = e & 2 ? b1 : b0;
-    v0[e] = (e & 1 ? wa >> 16 : wa & 0xffffu) >= d.thresh ? v0[e] * d.scale : 0.f;
-    v1[e] = (e & 1 ? wb >> 16 : wb & 0xffffu) >= d.thresh ? v1[e] * d.scale : 0.f;
-  }
-}
-
-
 template <typename T, int V, int TH, bool WHOLE> __global__ __launch_bounds__(TH) void norm_chunk_apply_kernel(const NormArgs a) {
   constexpr int U = 4, W = WHOLE ? 1 : V;
   typedef Batch<T, V, U> B;
@@ -672,7 +692,8 @@ template <int TH> __device__ __forceinline__ void team_group_sums(const NormArgs
 }
 
 // The whole backward pass of a span in registers, x and dy read once: (A, B) of its channels go to ab[image][channel] for the parameters'
-// gradients over the images.
+// gradients over the images.  dz stays in registers as float32 between the sums and dx (dropout and the activation's gradient are half of the
+// arithmetic: 32 x 48 x 48 x 128 bfloat16 took 33 us with both computed twice).
 template <typename T, int V, int R, int TH, bool WHOLE> __global__ __launch_bounds__(TH) void norm_team_grad_kernel(const NormArgs a) {
   __shared__ float2 sum[TH * V];
   __shared__ float2 tot[TH * V];
@@ -689,19 +710,25 @@ template <typename T, int V, int R, int TH, bool WHOLE> __global__ __launch_boun
   NormChan<V, WHOLE> ch;
   ch.load(a, t.img, t.c0, t.on);
   const uint64_t offset = a.drop.thresh ? drop_offset(a.drop) : 0;
-  float sa[V], sb[V];
+  float sa[V], sb[V], dz[R][V];
 #pragma unroll
   for (int e = 0; e < V; ++e) sa[e] = sb[e] = 0.f;
 #pragma unroll
+  for (int r = 0; r < R; ++r) g[r].widen(dz[r]);
+  if (a.drop.thresh && t.on) {
+    const bool pairs = V == 4 && a.span % 8 == 0;
+#pragma unroll
+    for (int r = 0; r < R; r += 2)
+      if (t.row + r * a.rows < a.p) drop_two<V>(dz[r], dz[r + 1 < R ? r + 1 : r], r + 1 < R ? 2 : 1, pairs && r + 1 < R, i0 + r * di, di, a.drop, offset);
+  }
+#pragma unroll
   for (int r = 0; r < R; ++r)
     if (t.on && t.row + r * a.rows < a.p) {
-      float v[V], w[V];
+      float v[V];
       q[r].widen(v);
-      g[r].widen(w);
-      if (a.drop.thresh) drop_apply<V>(w, i0 + r * di, a.drop, offset);
-      norm_dz<V, WHOLE>(a, ch, v, w);
+      norm_dz<V, WHOLE>(a, ch, v, dz[r]);
 #pragma unroll
-      for (int e = 0; e < V; ++e) { sa[e] += w[e]; sb[e] += w[e] * v[e]; }
+      for (int e = 0; e < V; ++e) { sa[e] += dz[r][e]; sb[e] += dz[r][e] * v[e]; }
     }
 #pragma unroll
   for (int e = 0; e < V; ++e) sb[e] *= ch.rstd[WHOLE ? 0 : e];
@@ -710,7 +737,7 @@ template <typename T, int V, int R, int TH, bool WHOLE> __global__ __launch_boun
   for (int c = threadIdx.x; c < a.span; c += TH) a.ab[(size_t)t.img * a.c + t.cbase + c] = sum[c];
   __syncthreads();
 #pragma unroll
-  for (int r = 0; r < R; ++r) { q[r].keep(); g[r].keep(); }
+  for (int r = 0; r < R; ++r) q[r].keep();
   if (!t.on) return;
   NormBack<V, WHOLE> back;
 #pragma unroll
@@ -718,13 +745,12 @@ template <typename T, int V, int R, int TH, bool WHOLE> __global__ __launch_boun
 #pragma unroll
   for (int r = 0; r < R; ++r)
     if (t.row + r * a.rows < a.p) {
-      float v[V], w[V];
+      float v[V];
       q[r].widen(v);
-      g[r].widen(w);
-      if (a.drop.thresh) drop_apply<V>(w, i0 + r * di, a.drop, offset);
-      norm_dz<V, WHOLE>(a, ch, v, w);
-      back.apply(ch, v, w);
-      store_v<T, V>(dx.ptr(r), w);
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] -= ch.mean[WHOLE ? 0 : e];
+      back.apply(ch, v, dz[r]);
+      store_v<T, V>(dx.ptr(r), dz[r]);
     }
 }
 
