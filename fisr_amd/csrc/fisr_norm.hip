@@ -132,12 +132,13 @@ bool two_tiling(NormArgs& a, int v, int elem_bytes, bool backward) {
   // (no such span, or one of few columns with more channels beside it: workgroups of any channels read whole lines)
   if (k == 0 || (k < most && k * unit / v < 64)) return false;
   set_team(a, v, 256, k * unit);
-  // First launch: two long-lived workgroups a CU, whose numbers have to be joined.  Second: six a CU; of tensors beyond 192 MB pieces of 24 KB, or
-  // eight times what a workgroup reads to join the first one's numbers.
+  // First launch: two long-lived workgroups a CU, whose numbers have to be joined.  Second: four a CU, six above 48 MB (272 x 496 x 128 bfloat16,
+  // 35 MB: 30.9 us with four, 34.5 with six; 544 x 992 x 64, 69 MB: 48.9 and 47.2); of tensors beyond 192 MB pieces of 24 KB, or eight times what a
+  // workgroup reads to join the first one's numbers.
   const size_t bytes = (size_t)a.n * a.p * a.c * elem_bytes * (backward ? 2 : 1);
   chunks_for(a, env_int("NORM_SWG", 512), least_chunk(v), a.chunks, a.ppc);
   a.join = a.chunks * (a.span / a.d) <= 2048;
-  size_t second = 1536;
+  size_t second = bytes > (size_t)48 << 20 ? 1536 : 1024;
   if (bytes > (size_t)192 << 20) second = std::min<size_t>(bytes / std::max(24576, (backward || a.join) * a.chunks * (a.span / a.d) * 64), 32768);
   chunks_for(a, env_int("NORM_AWG", (int)second), least_chunk(v), a.achunks, a.appc);
   return true;
