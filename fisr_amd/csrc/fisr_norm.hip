@@ -18,7 +18,6 @@ using namespace fisr;
 
 namespace {
 
-
 #ifdef FISR_DIAG
 int env_int(const char* name, int def) { const char* e = getenv(name); return e ? atoi(e) : def; }
 #else
@@ -35,14 +34,14 @@ void chunks_for(const NormArgs& a, int workgroups, int least, int& chunks, int& 
 // 2 x 40 x 50 x 9 bfloat16 in 8.8 at 1024 elements, 14.0 at 8192)
 constexpr int LEAST_ELEMENTS = 1024;
 constexpr int least_chunk(int v) { return v * 512 > LEAST_ELEMENTS ? v * 512 : LEAST_ELEMENTS; }
-constexpr int MOST_CHUNK_GROUPS = 2048;                          // of a batch, by chunks_for: what the workspace is made for
+constexpr int MOST_WORKGROUPS = 2048;                          // of a batch, by chunks_for: what the workspace is made for
 
 // Workspace: `part` of n * chunks * c float2, and for the backward pass s12 of n * groups * chunks and ab of n * c.  Not a function of the
 // vector width or the form that runs: its size is asked for without the tensors.
 struct WsLayout { size_t part, s12, ab; };
 WsLayout ws_layout(const NormArgs& a, bool backward) {
   int chunks, ppc;
-  chunks_for(a, MOST_CHUNK_GROUPS, LEAST_ELEMENTS, chunks, ppc);
+  chunks_for(a, MOST_WORKGROUPS, LEAST_ELEMENTS, chunks, ppc);
   WsLayout w{(size_t)a.n * chunks * a.c, 0, 0};
   if (backward) { w.s12 = (size_t)a.n * a.groups * chunks; w.ab = (size_t)a.n * a.c; }
   return w;
@@ -91,9 +90,9 @@ int team_variant(NormArgs& a, int v, int elem_bytes, bool backward) {
   const int line = env_int("NORM_LINE", elems * elem_bytes > (size_t)4 << 20 ? 64 : 16);  // least bytes of a span: narrow ones read a cache line many times over
   int best = -1, best_span = 0;
   for (int k = 1; k <= most; ++k) {
-    if (most % k) continue;
     const int span = k * unit, cols = span / v;
     if (cols > 256) break;
+    if (most % k) continue;
     if (best >= 0 && best_span * elem_bytes >= line && (best_span * elem_bytes >= 128 || (long long)a.n * (a.c / span) < 512)) break;
     int fit = -1;
     for (int i = 0; i < (int)(sizeof(TEAM) / sizeof(TEAM[0])) && fit < 0; ++i) {
@@ -127,19 +126,21 @@ template <typename T, int V> void launch_team(const NormArgs& a, bool backward, 
 bool two_tiling(NormArgs& a, int v, int elem_bytes, bool backward) {
   if (wide_strides(a, 256, elem_bytes)) return false;
   const int unit = span_unit(a, v), most = a.c / unit;
-  int k = most;
-  while (k > 0 && (most % k || k * unit / v > 256)) --k;
+  int k = std::min(most, 256 * v / unit);
+  while (k > 0 && most % k) --k;
   // (no such span, or one of few columns with more channels beside it: workgroups of any channels read whole lines)
   if (k == 0 || (k < most && k * unit / v < 64)) return false;
   set_team(a, v, 256, k * unit);
   // First launch: two long-lived workgroups a CU, whose numbers have to be joined.  Second: four a CU, six above 48 MB (272 x 496 x 128 bfloat16,
-  // 35 MB: 30.9 us with four, 34.5 with six; 544 x 992 x 64, 69 MB: 48.9 and 47.2); of tensors beyond 192 MB pieces of 24 KB, or eight times what a
-  // workgroup reads to join the first one's numbers.
+  // 35 MB: 30.9 us with four, 34.5 with six; 544 x 992 x 64, 69 MB: 48.9 and 47.2); beyond 192 MB pieces of 48 KB, backward 64, at most 64 a CU (twelve
+  // 544 x 992 x 64 float16: 407 us in 16384 pieces, 443 in 1536, 422 in 32768; backward 702, 721, 767), or eight times what a workgroup reads to
+  // join the first launch's numbers.
   const size_t bytes = (size_t)a.n * a.p * a.c * elem_bytes * (backward ? 2 : 1);
   chunks_for(a, env_int("NORM_SWG", 512), least_chunk(v), a.chunks, a.ppc);
-  a.join = a.chunks * (a.span / a.d) <= 2048;
+  // (272 x 496 x 128 in 32 groups, backward: 51 us with norm_grad_join_kernel for the 16384 numbers, 60 without; in 512 groups 49 and 626)
+  a.join = a.chunks * (a.span / a.d) <= env_int("NORM_JOIN", 2048);
   size_t second = bytes > (size_t)48 << 20 ? 1536 : 1024;
-  if (bytes > (size_t)192 << 20) second = std::min<size_t>(bytes / std::max(24576, (backward || a.join) * a.chunks * (a.span / a.d) * 64), 32768);
+  if (bytes > (size_t)192 << 20) second = std::min<size_t>(bytes / std::max(backward ? 65536 : 49152, a.join * a.chunks * (a.span / a.d) * 64), 16384);
   chunks_for(a, env_int("NORM_AWG", (int)second), least_chunk(v), a.achunks, a.appc);
   return true;
 }
@@ -150,6 +151,7 @@ template <typename T, int V, bool WHOLE> void launch_two_whole(const NormArgs& a
   if (backward) {
     const int pblocks = a.dgamma || a.dbeta ? (a.c + 15) / 16 : 0;
     hipLaunchKernelGGL((norm_chunk_sums_kernel<T, V, TH, WHOLE>), g1, dim3(TH), 0, st, a);
+    if (!a.join) hipLaunchKernelGGL(norm_grad_join_kernel, dim3(a.n * a.groups), dim3(64), 0, st, a);
     hipLaunchKernelGGL((norm_chunk_grad_kernel<T, V, TH, WHOLE>), dim3(pblocks + a.n * a.achunks, ny), dim3(TH), 0, st, a, pblocks);
     return;
   }
@@ -175,7 +177,7 @@ template <typename T, int V> bool launch_two(NormArgs a, bool backward, hipStrea
 
 // Any shape.
 template <typename T, int V> void launch_any(NormArgs a, bool backward, hipStream_t st) {
-  chunks_for(a, MOST_CHUNK_GROUPS, 8192, a.chunks, a.ppc);
+  chunks_for(a, MOST_WORKGROUPS, 8192, a.chunks, a.ppc);
   const int cv = (a.c + V - 1) / V, ny = (cv + 255) / 256;
   a.cb = (cv + ny - 1) / ny;
   a.rows = 256 / a.cb;

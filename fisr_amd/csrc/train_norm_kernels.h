@@ -6,8 +6,7 @@
 //   backward: dz = drop(dy) * act'(z);  A[n,c] = sum_p dz,  B[n,c] = sum_p dz * xh;  dbeta = sum_n A,  dgamma = sum_n B
 //             dx = rstd * (dz * gamma - S1 / (P D) - xh * S2 / (P D)),  S1[n,g] = sum_{c in g} gamma A,  S2 = sum gamma B
 //
-// Every sum, statistic and intermediate is float32 (the merges over workgroups float64); only y and dx are rounded, once, to the
-// tensors' type.  There are no atomics: partial results go through the workspace and are joined in a fixed order, so a call's
+// Every sum, statistic and intermediate is float32 or more; only y and dx are rounded, once, to the tensors' type.  There are no atomics: partial results go through the workspace and are joined in a fixed order, so a call's
 // results are the same bits every time.
 #pragma once
 #include <hip/hip_runtime.h>
@@ -300,7 +299,6 @@ template <int V> __device__ __forceinline__ void drop_apply_pair(float (&v0)[V],
   }
 }
 
-
 // Dropout of the K = 1 or 2 vectors v of a thread, elements i and i + di on.  pairs: drop_apply_pair may be used.
 template <int V> __device__ __forceinline__ void drop_two(float (&v0)[V], float (&v1)[V], int k, bool pairs, uint64_t i, uint64_t di, const DropArgs& d, uint64_t offset) {
   if constexpr (V == 4) {
@@ -465,7 +463,7 @@ template <typename T, int V, int U> __device__ __forceinline__ void stats_batch(
 
 // The vectors of a thread in a chunk, U at a time, the next ones on their way while these are worked on: two buffers in turn (a copy between
 // them would cost as many instructions as a vector's arithmetic).  `load(buffer, r, m)` and `work(buffer, r, m)` take vectors r .. r + m - 1;
-// m is U but for the last ones.  begin() loads the first, finish() does the rest.
+// m is U but for the last ones.  fetch() loads the first, finish() does the rest.
 template <int U, typename B> struct Chunk {
   int full, tail;
   B b0, b1;
@@ -840,6 +838,25 @@ __device__ __forceinline__ void param_grads(const NormArgs& a, const float2* ab,
 }
 __global__ __launch_bounds__(256) void norm_params_kernel(const NormArgs a, const float2* ab, int rows) { param_grads(a, ab, rows, blockIdx.x); }
 
+// Sums over `chunks` numbers of each of `groups` groups: 2^jl lanes a group, all groups at once
+template <int TH> __device__ __forceinline__ void join_sums(const float2* part, int chunks, int groups, int jl, float2* out) {
+  const int lanes = 1 << jl, lane = threadIdx.x & (lanes - 1);
+  for (int j0 = 0; j0 < groups; j0 += TH >> jl) {
+    const int j = j0 + (threadIdx.x >> jl);
+    float s1 = 0.f, s2 = 0.f;
+    if (j < groups) {
+#pragma unroll 4
+      for (int k = lane; k < chunks; k += lanes) { const float2 f = part[(size_t)j * chunks + k]; s1 += f.x; s2 += f.y; }
+    }
+    for (int k = lanes >> 1; k; k >>= 1) { s1 += __shfl_xor(s1, k); s2 += __shfl_xor(s2, k); }
+    if (j < groups && lane == 0) out[j] = make_float2(s1, s2);
+  }
+}
+// a wave a group of the whole batch, into ab[image][group]
+__global__ __launch_bounds__(64) void norm_grad_join_kernel(const NormArgs a) {
+  join_sums<64>(a.s12 + (size_t)blockIdx.x * a.chunks, a.chunks, 1, 6, a.ab + blockIdx.x);
+}
+
 // Second launch: dx.  Its first `pblocks` workgroups sum the parameters' gradients instead.
 template <typename T, int V, int TH, bool WHOLE> __global__ __launch_bounds__(TH) void norm_chunk_grad_kernel(const NormArgs a, int pblocks) {
   static_assert(TH == 256, "param_grads");
@@ -858,21 +875,14 @@ template <typename T, int V, int TH, bool WHOLE> __global__ __launch_bounds__(TH
   if (t.on) c.fetch(c.b0, 0, load);
   NormChan<V, WHOLE> ch;
   ch.load(a, t.img, t.c0, t.on);
-  {
-    const int lanes = 1 << a.jl, lane = threadIdx.x & (lanes - 1), groups = a.span / a.d;
-    for (int j0 = 0; j0 < groups; j0 += TH >> a.jl) {
-      const int j = j0 + (threadIdx.x >> a.jl);
-      float s1 = 0.f, s2 = 0.f;
-      if (j < groups) {
-        const float2* part = a.s12 + ((size_t)t.img * a.groups + t.cbase / a.d + j) * a.chunks;
-#pragma unroll 4
-        for (int k = lane; k < a.chunks; k += lanes) { const float2 f = part[k]; s1 += f.x; s2 += f.y; }
-      }
-      for (int k = lanes >> 1; k; k >>= 1) { s1 += __shfl_xor(s1, k); s2 += __shfl_xor(s2, k); }
-      if (j < groups && lane == 0) tot[j] = make_float2(s1, s2);
-    }
-    __syncthreads();
+  const size_t g0 = (size_t)t.img * a.groups + div_by(t.cbase, a.by_d);
+  const int groups = div_by(a.span, a.by_d);
+  if (a.join) {
+    join_sums<TH>(a.s12 + g0 * a.chunks, a.chunks, groups, a.jl, tot);
+  } else {
+    for (int j = threadIdx.x; j < groups; j += TH) tot[j] = a.ab[g0 + j];
   }
+  __syncthreads();
   if (!t.on) return;
   NormBack<V, WHOLE> back;
 #pragma unroll
