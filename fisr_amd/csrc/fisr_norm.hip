@@ -176,20 +176,27 @@ template <typename T, int V> bool launch_two(NormArgs a, bool backward, hipStrea
 }
 
 // Any shape.
+constexpr int JOIN_WIDE = 4096;                                // numbers a group from which its join takes 1024 threads (4 x 64 x 64 x 1031 float32,
+                                                               // one group: 72 us, backward 96; 256 threads 252 and 188)
 template <typename T, int V> void launch_any(NormArgs a, bool backward, hipStream_t st) {
-  chunks_for(a, MOST_WORKGROUPS, 8192, a.chunks, a.ppc);
   const int cv = (a.c + V - 1) / V, ny = (cv + 255) / 256;
+  // (divided by ny: what the joins read is chunks * channels a group.  4 x 64 x 64 x 1031 float32 with joins of 256 threads, one group: 252 us, 1216
+  // undivided; 1031 groups: 51 and 90; half as many chunks again 167 and 64)
+  chunks_for(a, std::max(a.n, MOST_WORKGROUPS / ny), 8192, a.chunks, a.ppc);
   a.cb = (cv + ny - 1) / ny;
   a.rows = 256 / a.cb;
-  const dim3 grid(a.n * a.chunks, ny);
+  const dim3 grid(a.n * a.chunks, ny), joins(a.n * a.groups);
+  const bool wide = a.chunks * a.d > JOIN_WIDE;
   if (!backward) {
     hipLaunchKernelGGL((norm_stats_kernel<T, V>), grid, dim3(256), 0, st, a);
-    hipLaunchKernelGGL(norm_stats_join_kernel, dim3(a.n * a.groups), dim3(256), 0, st, a);
+    if (wide) hipLaunchKernelGGL(norm_stats_join_kernel<1024>, joins, dim3(1024), 0, st, a);
+    else hipLaunchKernelGGL(norm_stats_join_kernel<256>, joins, dim3(256), 0, st, a);
     hipLaunchKernelGGL((norm_apply_kernel<T, V>), grid, dim3(256), 0, st, a);
     return;
   }
   hipLaunchKernelGGL((norm_bwd_sums_kernel<T, V>), grid, dim3(256), 0, st, a);
-  hipLaunchKernelGGL(norm_bwd_join_kernel, dim3(a.n * a.groups), dim3(256), 0, st, a);
+  if (wide) hipLaunchKernelGGL(norm_bwd_join_kernel<1024>, joins, dim3(1024), 0, st, a);
+  else hipLaunchKernelGGL(norm_bwd_join_kernel<256>, joins, dim3(256), 0, st, a);
   hipLaunchKernelGGL((norm_bwd_apply_kernel<T, V>), grid, dim3(256), 0, st, a);
   if (a.dgamma || a.dbeta) hipLaunchKernelGGL(norm_params_kernel, dim3((a.c + 15) / 16), dim3(256), 0, st, a, a.ab, a.n);
 }

@@ -299,17 +299,63 @@ template <int V> __device__ __forceinline__ void drop_apply_pair(float (&v0)[V],
   }
 }
 
-// Dropout of the K = 1 or 2 vectors v of a thread, elements i and i + di on.  pairs: drop_apply_pair may be used.
-template <int V> __device__ __forceinline__ void drop_two(float (&v0)[V], float (&v1)[V], int k, bool pairs, uint64_t i, uint64_t di, const DropArgs& d, uint64_t offset) {
-  if constexpr (V == 4) {
-    if (pairs) {
-      drop_apply_pair<V>(v0, v1, i, i + di, d, offset);      // (the second may be no pixel: nobody uses it)
-      return;
+// Which elements of a thread's R vectors dropout keeps, found while the vectors are on their way: the generator's numbers need none of them
+// (32 x 48 x 48 x 128 bfloat16: 18.7 us against 19.7 with the numbers made where they are used, backward 24.7 and 26.5).  It stands before any other
+// load of the kernel: with gamma's and beta's under way the compiler took one of their registers for a product and waited for all loads first.
+// Bit (e >> 1) + 16 (e & 1) + 4 (r & 3) of bits[r >> 2] is element e of vector r: a word of the generator is two elements, and packed 16-bit
+// operations make both bits at once, max(number - (thresh - 1), 0) and min(that, 1).
+template <int V, int R> struct DropMask {
+  uint32_t bits[(R + 3) / 4];
+  static __device__ __forceinline__ uint32_t two(uint32_t word, uint32_t below) {
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    const u16x2 b = {(unsigned short)below, (unsigned short)below}, one = {1, 1};
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_elementwise_sub_sat(__builtin_bit_cast(u16x2, word), b), one));
+  }
+  __device__ __forceinline__ void put(int r, uint32_t m) { bits[r >> 2] |= m << 4 * (r & 3); }
+  // vector r is elements i0 + r * di on; pairs: as drop_apply_pair's; `pixel(r)`: whether there is a vector r
+  template <typename F> __device__ __forceinline__ void find(bool pairs, uint64_t i0, uint64_t di, const DropArgs& d, uint64_t offset, F pixel) {
+    const uint32_t below = d.thresh - 1;
+#pragma unroll
+    for (int k = 0; k < (R + 3) / 4; ++k) bits[k] = 0;
+    if (V == 4 && pairs && R > 1) {
+      const bool odd = threadIdx.x & 1;
+      uint64_t i = i0 + (odd ? di : 0);
+#pragma unroll
+      for (int r = 0; r < R; r += 2, i += 2 * di)
+        if (pixel(r)) {                                      // (vector r + 1 may be no pixel: nobody uses it)
+          const Philox n = philox7(i >> 3, offset, d.seed);
+          const uint32_t lo = two(n.w[0], below) | two(n.w[1], below) << 1, hi = two(n.w[2], below) | two(n.w[3], below) << 1;
+          const uint32_t got = __builtin_amdgcn_mov_dpp(odd ? lo : hi, 0xB1, 0xf, 0xf, true);               // quad_perm 1, 0, 3, 2
+          put(r, odd ? got : lo);
+          if (r + 1 < R) put(r + 1, odd ? hi : got);
+        }
+    } else {
+      uint64_t i = i0;
+#pragma unroll
+      for (int r = 0; r < R; ++r, i += di)
+        if (pixel(r)) {
+          const Philox n = philox7(i >> 3, offset, d.seed);
+          if (V == 8) {
+            put(r, two(n.w[0], below) | two(n.w[1], below) << 1 | two(n.w[2], below) << 2 | two(n.w[3], below) << 3);
+          } else {
+            const int at = (int)(i & 7);
+            const uint32_t lo = at & 4 ? n.w[2] : n.w[0], hi = at & 4 ? n.w[3] : n.w[1];
+            if (V == 4) put(r, two(lo, below) | two(hi, below) << 1);
+            else put(r, two((at & 2 ? hi : lo) >> (V == 1 && (at & 1) ? 16 : 0), below) & (V == 1 ? 1u : ~0u));
+          }
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < (R + 3) / 4; ++k) asm volatile("" : "+v"(bits[k]));      // (here, not where they are used)
+  }
+  __device__ __forceinline__ void apply(int r, float (&v)[V], float scale) const {
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const int bit = (e >> 1) + 16 * (e & 1) + 4 * (r & 3);
+      v[e] = __builtin_bit_cast(float, __builtin_bit_cast(int, v[e] * scale) & (int)(bits[r >> 2] << (31 - bit)) >> 31);
     }
   }
-  drop_apply<V>(v0, i, d, offset);
-  if (k > 1) drop_apply<V>(v1, i + di, d, offset);
-}
+};
 
 // ---- one launch, one read: a workgroup holds `span` channels (whole groups) of all pixels of an image in registers ----
 // Thread (row, col) keeps the vectors of column col at the pixels row + r * rows, r < R, as they were loaded (16-bit tensors packed).
@@ -351,6 +397,10 @@ template <typename T, int V> struct Walk {
     }
   }
 };
+// Bound by the phases, which wait for each other (all loads, two sums over the workgroup, all stores, one workgroup a CU for the largest), and
+// by a span being a part of a cache line, which the workgroups of an image read from L2 in turn: 32 x 48 x 48 x 128 bfloat16 in 32 groups, 38 MB, 17.0 us
+// without dropout, 17.8 with, 6.3 at the rate of a copy; the two launches below take 24.0 and 25.7.  Twice as large it is 29.0 and 28.8, so up to
+// 16 M elements go here.
 template <typename T, int V, int R, int TH> __global__ __launch_bounds__(TH) void norm_team_kernel(const NormArgs a) {
   __shared__ float red[TH * V];
   __shared__ float tot[2][TH * V];                           // (as many groups as channels at the most)
@@ -360,6 +410,10 @@ template <typename T, int V, int R, int TH> __global__ __launch_bounds__(TH) voi
 #pragma unroll
   for (int r = 0; r < R; ++r)
     if (t.on && t.row + r * a.rows < a.p) q[r].load(x.ptr(r));
+  DropMask<V, R> drop;
+  if (a.drop.thresh && t.on)
+    drop.find(a.span % 8 == 0, ((uint64_t)t.img * a.p + t.row) * a.c + t.c0, (uint64_t)a.rows * a.c, a.drop, drop_offset(a.drop),
+              [&](int r) { return t.row + r * a.rows < a.p; });
   float gamma[V], beta[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) {
@@ -398,31 +452,24 @@ template <typename T, int V, int R, int TH> __global__ __launch_bounds__(TH) voi
   if (!t.on) return;
 #pragma unroll
   for (int e = 0; e < V; ++e) gamma[e] *= tot[1][div_by(t.col * V + e, a.by_d)];
-  const uint64_t offset = a.drop.thresh ? drop_offset(a.drop) : 0;
-  const uint64_t i0 = ((uint64_t)t.img * a.p + t.row) * a.c + t.c0, di = (uint64_t)a.rows * a.c;
-  const bool pairs = V == 4 && a.span % 8 == 0;
 #pragma unroll
-  for (int r = 0; r < R; r += 2)
+  for (int r = 0; r < R; ++r)
     if (t.row + r * a.rows < a.p) {
-      float v[2][V];
-      const int m = r + 1 < R && t.row + (r + 1) * a.rows < a.p ? 2 : 1;
+      float v[V];
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
-        if (r + k < R && k < m) {
-#pragma unroll
-          for (int e = 0; e < V; ++e) v[k][e] = (q[r + k < R ? r + k : r].get(e) - mean[e]) * gamma[e] + beta[e];
-          act_apply<V>(v[k], a.act);
-        }
-      if (a.drop.thresh) drop_two<V>(v[0], v[1], m, pairs, i0 + r * di, di, a.drop, offset);
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-        if (r + k < R && k < m) store_v<T, V>(y.ptr(r + k), v[k]);
+      for (int e = 0; e < V; ++e) v[e] = (q[r].get(e) - mean[e]) * gamma[e] + beta[e];
+      act_apply<V>(v, a.act);
+      if (a.drop.thresh) drop.apply(r, v, a.drop.scale);
+      store_v<T, V>(y.ptr(r), v);
     }
 }
 
 // ---- two launches, one read each: statistics per group and chunk of pixels, then the output ----
 // part[image][group][chunk] = (mean, M2) of a chunk.  The second launch's workgroups join their image's chunks themselves, or, where that is
 // much to read for each of them (few images with many chunks), norm_join_kernel joins them once in between.
+// Bound by memory where the tensor is beyond the caches: 12 x 544 x 992 x 64 float16, 829 MB, statistics 129 us (6.4 TB/s), output 279 us (5.9 TB/s; the
+// best copy of this card 6.0).  Between (75 MB: 15.1 and 23.5 us, 5.0 and 6.4 TB/s) the first launch's ramp and tail count as well, and
+// with gelu on 69 MB the arithmetic does (26.5 us for 138 MB).  The parts cannot be one launch without waiting for all workgroups of an image.
 template <int V> __device__ __forceinline__ NormTeam chunk_team(const NormArgs& a, int block, int chunks, int ppc, int& chunk, int& p0, int& p1) {
   NormTeam t;
   t.img = block / chunks;
@@ -691,13 +738,13 @@ template <int TH> __device__ __forceinline__ void team_group_sums(const NormArgs
 
 // The whole backward pass of a span in registers, x and dy read once: (A, B) of its channels go to ab[image][channel] for the parameters'
 // gradients over the images.  dz stays in registers as float32 between the sums and dx (dropout and the activation's gradient are half of the
-// arithmetic: 32 x 48 x 48 x 128 bfloat16 took 33 us with both computed twice).
+// arithmetic: 32 x 48 x 48 x 128 bfloat16 took 33 us with both computed twice).  Bound as the forward pass is: 57 MB in 23.3 us, 24.3 with dropout (the
+// two launches 38.9 and 40.1), 9.4 at the rate of a copy.
 template <typename T, int V, int R, int TH, bool WHOLE> __global__ __launch_bounds__(TH) void norm_team_grad_kernel(const NormArgs a) {
   __shared__ float2 sum[TH * V];
   __shared__ float2 tot[TH * V];
   const NormTeam t = span_team<V>(a);
   const Walk<T, V> x(a, t, a.x, a.xcs, 0), dy(a, t, a.dy, a.dycs, 0), dx(a, t, a.y, a.ycs, 0);
-  const uint64_t i0 = ((uint64_t)t.img * a.p + t.row) * a.c + t.c0, di = (uint64_t)a.rows * a.c;
   Pack<T, V> q[R], g[R];
 #pragma unroll
   for (int r = 0; r < R; ++r)
@@ -705,25 +752,22 @@ template <typename T, int V, int R, int TH, bool WHOLE> __global__ __launch_boun
       q[r].load(x.ptr(r));
       g[r].load(dy.ptr(r));
     }
+  DropMask<V, R> drop;
+  if (a.drop.thresh && t.on)
+    drop.find(a.span % 8 == 0, ((uint64_t)t.img * a.p + t.row) * a.c + t.c0, (uint64_t)a.rows * a.c, a.drop, drop_offset(a.drop),
+              [&](int r) { return t.row + r * a.rows < a.p; });
   NormChan<V, WHOLE> ch;
   ch.load(a, t.img, t.c0, t.on);
-  const uint64_t offset = a.drop.thresh ? drop_offset(a.drop) : 0;
   float sa[V], sb[V], dz[R][V];
 #pragma unroll
   for (int e = 0; e < V; ++e) sa[e] = sb[e] = 0.f;
-#pragma unroll
-  for (int r = 0; r < R; ++r) g[r].widen(dz[r]);
-  if (a.drop.thresh && t.on) {
-    const bool pairs = V == 4 && a.span % 8 == 0;
-#pragma unroll
-    for (int r = 0; r < R; r += 2)
-      if (t.row + r * a.rows < a.p) drop_two<V>(dz[r], dz[r + 1 < R ? r + 1 : r], r + 1 < R ? 2 : 1, pairs && r + 1 < R, i0 + r * di, di, a.drop, offset);
-  }
 #pragma unroll
   for (int r = 0; r < R; ++r)
     if (t.on && t.row + r * a.rows < a.p) {
       float v[V];
       q[r].widen(v);
+      g[r].widen(dz[r]);
+      if (a.drop.thresh) drop.apply(r, dz[r], a.drop.scale);
       norm_dz<V, WHOLE>(a, ch, v, dz[r]);
 #pragma unroll
       for (int e = 0; e < V; ++e) { sa[e] += dz[r][e]; sb[e] += dz[r][e] * v[e]; }
@@ -775,6 +819,7 @@ template <typename T, int V, bool WHOLE> struct GradPixels {
   }
 };
 
+// Bound by memory: 32 x 96 x 96 x 64 float32, 75 MB a tensor, first launch 30.7 us (4.9 TB/s), second 36.9 us (6.1 TB/s).
 // First launch: part[image][chunk][channel] = (A, B) of a chunk, and behind it s12[image][group][chunk] = (sum of gamma A, of gamma B) / (P D).
 template <typename T, int V, int U> struct GradBuffer { Pack<T, V> x[U], dy[U]; };
 template <typename T, int V, int TH, bool WHOLE> __global__ __launch_bounds__(TH) void norm_chunk_sums_kernel(const NormArgs a) {
@@ -906,7 +951,8 @@ template <typename T, int V, int TH, bool WHOLE> __global__ __launch_bounds__(TH
 }
 
 // ---- any shape: workgroups of any channels, three launches (four backward).  What the forms above do not take: pixels of more vectors
-// than a workgroup has threads ----
+// than a workgroup has threads.  4 x 64 x 64 x 1031 float32 (68 MB): 53 us in 1031 groups, 72 in one, where one workgroup an image joins the chunks;
+// backward 97 and 96.  Scalar accesses, as the odd channels want them, bound the rest ----
 struct NormTile {
   int img, chunk, p0, p1, row, c0;
   bool on;
@@ -958,35 +1004,43 @@ template <typename T, int V> __global__ __launch_bounds__(256) void norm_stats_k
   }
 }
 
-__device__ __forceinline__ double block_sum(double v, double* red) {            // 256 threads; the same value for every thread
+template <int TH> __device__ __forceinline__ double block_sum(double v, double* red) {            // red: TH / 64 numbers; the same value for every thread
 #pragma unroll
   for (int s = 32; s; s >>= 1) v += __shfl_xor(v, s);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
-  return (red[0] + red[1]) + (red[2] + red[3]);
+  v = 0.0;
+#pragma unroll
+  for (int k = 0; k < TH / 64; ++k) v += red[k];
+  return v;
 }
 
-// ---- statistics, second half: one workgroup per (image, group) joins the chunks' (mean, M2) of its channels ----
-__global__ __launch_bounds__(256) void norm_stats_join_kernel(const NormArgs a) {
-  __shared__ double red[4];
+// ---- statistics, second half: one workgroup per (image, group) joins the chunks' (mean, M2) of its channels: nd channels beside each other,
+// `lanes` chunks at once.  Bound by its loads' latency where there are few groups: 1024 threads there. ----
+template <int TH> __global__ __launch_bounds__(TH) void norm_stats_join_kernel(const NormArgs a) {
+  __shared__ double red[TH / 64];
   const int img = blockIdx.x / a.groups, g = blockIdx.x - img * a.groups;
   const float2* part = a.part + (size_t)img * a.chunks * a.c + (size_t)g * a.d;
-  const int total = a.chunks * a.d;
+  const int nd = min(TH, a.d), lanes = TH / nd, k0 = threadIdx.x / nd, ch0 = threadIdx.x - k0 * nd;
   const double m = (double)a.p * a.d;
   double s = 0.0;
-  for (int i = threadIdx.x; i < total; i += 256) {
-    const int k = i / a.d, ch = i - k * a.d;
-    s += (double)part[(size_t)k * a.c + ch].x * min(a.ppc, a.p - k * a.ppc);
-  }
-  const double mean = block_sum(s, red) / m;
+  if (k0 < lanes)
+    for (int ch = ch0; ch < a.d; ch += nd) {
+#pragma unroll 8
+      for (int k = k0; k < a.chunks; k += lanes) s += (double)part[(size_t)k * a.c + ch].x * min(a.ppc, a.p - k * a.ppc);
+    }
+  const double mean = block_sum<TH>(s, red) / m;
   double q = 0.0;
-  for (int i = threadIdx.x; i < total; i += 256) {
-    const int k = i / a.d, ch = i - k * a.d;
-    const float2 f = part[(size_t)k * a.c + ch];
-    q += (double)f.y + ((double)f.x - mean) * ((double)f.x - mean) * min(a.ppc, a.p - k * a.ppc);
-  }
-  const double var = block_sum(q, red) / m;
+  if (k0 < lanes)
+    for (int ch = ch0; ch < a.d; ch += nd) {
+#pragma unroll 8
+      for (int k = k0; k < a.chunks; k += lanes) {
+        const float2 f = part[(size_t)k * a.c + ch];
+        q += (double)f.y + ((double)f.x - mean) * ((double)f.x - mean) * min(a.ppc, a.p - k * a.ppc);
+      }
+    }
+  const double var = block_sum<TH>(q, red) / m;
   if (threadIdx.x == 0) {
     a.mean[blockIdx.x] = (float)mean;
     a.rstd[blockIdx.x] = (float)(1.0 / sqrt(var + (double)a.eps));
@@ -1048,19 +1102,21 @@ template <typename T, int V> __global__ __launch_bounds__(256) void norm_bwd_sum
 }
 
 // ---- backward, join: one workgroup per (image, group): (A, B) of its channels over the chunks, then S1, S2 ----
-__global__ __launch_bounds__(256) void norm_bwd_join_kernel(const NormArgs a) {
-  __shared__ double2 sum[256];
-  __shared__ double red[4];
+template <int TH> __global__ __launch_bounds__(TH) void norm_bwd_join_kernel(const NormArgs a) {
+  __shared__ double2 sum[TH];
+  __shared__ double red[TH / 64];
   const int img = blockIdx.x / a.groups, g = blockIdx.x - img * a.groups;
   double s1 = 0.0, s2 = 0.0;
-  for (int cb0 = 0; cb0 < a.d; cb0 += 256) {
-    const int nd = min(256, a.d - cb0), lanes = 256 / nd, k0 = threadIdx.x / nd, ch = threadIdx.x - k0 * nd;
+  for (int cb0 = 0; cb0 < a.d; cb0 += TH) {
+    const int nd = min(TH, a.d - cb0), lanes = TH / nd, k0 = threadIdx.x / nd, ch = threadIdx.x - k0 * nd;
     double sa = 0.0, sb = 0.0;
-    if (k0 < lanes)
+    if (k0 < lanes) {
+#pragma unroll 8
       for (int k = k0; k < a.chunks; k += lanes) {
         const float2 f = a.part[((size_t)img * a.chunks + k) * a.c + (size_t)g * a.d + cb0 + ch];
         sa += f.x; sb += f.y;
       }
+    }
     __syncthreads();
     sum[threadIdx.x] = make_double2(sa, sb);
     __syncthreads();
@@ -1074,7 +1130,7 @@ __global__ __launch_bounds__(256) void norm_bwd_join_kernel(const NormArgs a) {
     }
   }
   const double m = (double)a.p * a.d;
-  s1 = block_sum(s1, red); s2 = block_sum(s2, red);
+  s1 = block_sum<TH>(s1, red); s2 = block_sum<TH>(s2, red);
   if (threadIdx.x == 0) a.s12[blockIdx.x] = make_float2((float)(s1 / m), (float)(s2 / m));
 }
 

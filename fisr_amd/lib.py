@@ -87,14 +87,14 @@ def build(force: bool = False, verbose: bool = False, diag: bool = False, define
     if not diag and not out and not force and not needs_build():
         return SO_PATH
     os.makedirs(os.path.dirname(target), exist_ok=True)
-    flags = [hipcc_path(), "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden"]
+    flags = [hipcc_path(), "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden"] + \
+            (["-DFISR_DIAG"] if diag else []) + [f"-D{x}" for x in defines]
     with tempfile.TemporaryDirectory() as d:
         # fisr_api.hip's Winograd kernels write packed float32 instructions by hand; everything else is compiled without them
         norm_o = os.path.join(d, "fisr_norm.o")
         norm = flags + ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-c", "-o", norm_o, os.path.join(CSRC, "fisr_norm.hip")]
         cmd = flags + ["-shared", "-Wl,--version-script=" + os.path.join(CSRC, "exports.map"),
-                       f'-DFISR_SRC_HASH="{source_hash()}"'] + (["-DFISR_DIAG"] if diag else []) + [f"-D{x}" for x in defines] + \
-              ["-o", target, os.path.join(CSRC, "fisr_api.hip"), "-x", "none", norm_o]
+                       f'-DFISR_SRC_HASH="{source_hash()}"', "-o", target, os.path.join(CSRC, "fisr_api.hip"), "-x", "none", norm_o]
         if verbose:
             print(" ".join(norm), " ".join(cmd), sep="\n")
         subprocess.check_call(norm)
