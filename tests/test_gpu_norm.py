@@ -124,6 +124,12 @@ def test_group_norm_and_gradients_vs_oracle(env, shape, t, act, p):
     _within(_np(dx), dx64, edx, "dx")
 
 
+@pytest.mark.parametrize("t,act,p", KINDS[:3])
+@pytest.mark.parametrize("shape", [(2, 9, 11, 1031, 1), (1, 40, 25, 2062, 2), (2, 50, 40, 1031, 1)], ids=lambda s: "x".join(map(str, s)))
+def test_groups_of_more_channels_than_a_join_has_threads(env, shape, t, act, p):
+    test_group_norm_and_gradients_vs_oracle(env, shape, t, act, p)
+
+
 def test_mean_far_from_the_values_spread(env):
     """Values around 4096 with a spread of 1: a sum of squares about zero would lose all of it.  The bound of the docstring holds with
     X rstd = 4100."""
