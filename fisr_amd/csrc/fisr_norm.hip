@@ -3,6 +3,7 @@
 // fisr_api.hip write by hand.
 #include <cmath>
 #include <cstdlib>
+#include <initializer_list>
 
 #include "../../include/fisr.h"
 #include "host_util.h"
@@ -230,6 +231,21 @@ const char* drop_error(const fisr_dropout* d, DropArgs& out) {
   if ((uintptr_t)d->d_counter % 8) return "dropout: d_counter is not aligned to 8 bytes";
   return nullptr;
 }
+// The device that a call's operands are on, null ones aside; -1 where one is not memory of a GPU or of another one than those before it.  Every
+// pointer that a kernel goes to is among them: one to host memory would be a fault of the GPU.
+struct Operand { const char* name; const void* p; };
+int operands_device(std::initializer_list<Operand> operands, std::string& error) {
+  int dev = -1;
+  for (const Operand& o : operands) {
+    if (!o.p) continue;
+    const int d = device_of(o.p);
+    if (d < 0) error = std::string(o.name) + " is not memory of a GPU";
+    else if (dev >= 0 && d != dev) error = std::string(o.name) + " is memory of another GPU";
+    if (!error.empty()) return -1;
+    dev = d;
+  }
+  return dev;
+}
 size_t type_bytes(int type) { return type == FISR_TYPE_F32 ? 4 : type == FISR_TYPE_F16 || type == FISR_TYPE_BF16 ? 2 : 0; }
 
 int norm_call(const char* who, NormArgs& a, bool backward, int n, int h, int w, int c, int groups, int act, const fisr_dropout* drop, int type,
@@ -253,9 +269,10 @@ int norm_call(const char* who, NormArgs& a, bool backward, int n, int h, int w, 
   a.part = (float2*)ws;
   a.s12 = a.part + lay.part;
   a.ab = a.s12 + lay.s12;
-  const int dev = device_of(a.y);
-  if (dev < 0 || device_of(a.x) != dev || (backward && device_of(a.dy) != dev) || (ws && device_of(ws) != dev) || device_of(mean_rstd) != dev)
-    return bad("a pointer is not to memory of the output's device");
+  std::string error;
+  const int dev = operands_device({{"gamma", a.gamma}, {"beta", a.beta}, {"dgamma", a.dgamma}, {"dbeta", a.dbeta}, {"d_counter", a.drop.counter}, {"mean_rstd", mean_rstd},
+                                   {"the workspace", ws}, {"dy", a.dy}, {"x", a.x}, {backward ? "dx" : "y", a.y}}, error);
+  if (dev < 0) return bad(error.c_str());
   DeviceGuard guard(dev);
   NORM_HIP_OK(guard.err);
   const hipStream_t st = (hipStream_t)stream;
@@ -321,8 +338,9 @@ int fisr_train_dropout(const void* x, const void* residual, void* y, size_t coun
   if (count == 0) return 0;
   if (!x || !y) return bad("null tensor");
   if (((uintptr_t)x | (uintptr_t)residual | (uintptr_t)y) % es) return bad("a pointer is not aligned to its element");
-  const int dev = device_of(y);
-  if (dev < 0 || device_of(x) != dev || (residual && device_of(residual) != dev)) return bad("a pointer is not to memory of the output's device");
+  std::string error;
+  const int dev = operands_device({{"d_counter", d.counter}, {"residual", residual}, {"x", x}, {"y", y}}, error);
+  if (dev < 0) return bad(error.c_str());
   DeviceGuard guard(dev);
   NORM_HIP_OK(guard.err);
   const hipStream_t st = (hipStream_t)stream;

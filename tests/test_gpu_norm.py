@@ -382,3 +382,33 @@ def test_offsets_past_32_bits(env):
         got = _np(y[i, h - 1])
         assert np.abs(got - want[0, 0]).max() < 2.0 ** -8 * 6 + 1e-3, i
         assert np.array_equal(got == 0, want[0, 0] == 0)
+
+
+def test_c_entries_refuse_host_memory_beside_device_tensors(env):
+    """Whole calls on device tensors with one parameter, parameter gradient or counter in host memory: refused by name, outputs untouched."""
+    import ctypes
+    from fisr_amd import lib
+    torch, _ = env
+    L = lib.lib()
+    n, h, w, c, g = 2, 5, 6, 16, 4
+    x, dy, gamma, beta = _inputs(torch, n, h, w, c, "f32", 3)
+    y, st = torch.full_like(x, 7.0), torch.full((2, n, g), 7.0, device="cuda:0")
+    dg, db = torch.full_like(gamma, 7.0), torch.full_like(gamma, 7.0)
+    need = L.fisr_train_groupnorm_workspace_bytes(n, h, w, c, g, 1)
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda:0")
+    host = torch.ones(64)
+    stream = torch.cuda.current_stream().cuda_stream
+    dev = dict(gamma=gamma, beta=beta, dgamma=dg, dbeta=db, mean_rstd=st)
+    for name in (*dev, "d_counter"):
+        p = {k: (host if k == name else v).data_ptr() for k, v in dev.items()}
+        drop = ctypes.byref(lib.DropoutDesc(0.5, 1, 2, host.data_ptr() if name == "d_counter" else None))
+        if name not in ("dgamma", "dbeta"):
+            assert L.fisr_train_groupnorm(x.data_ptr(), c, p["gamma"], p["beta"], y.data_ptr(), c, p["mean_rstd"], n, h, w, c, g, 1e-5, 0, drop, 0, ws.data_ptr(),
+                                          need, stream) == -1
+            assert f"{name} is not memory of a GPU" in L.fisr_last_error(None).decode()
+        assert L.fisr_train_groupnorm_bwd(x.data_ptr(), c, dy.data_ptr(), c, p["gamma"], p["beta"], p["mean_rstd"], y.data_ptr(), c, p["dgamma"], p["dbeta"], 0, n,
+                                          h, w, c, g, 0, drop, 0, ws.data_ptr(), need, stream) == -1
+        assert f"{name} is not memory of a GPU" in L.fisr_last_error(None).decode()
+    assert L.fisr_train_dropout(x.data_ptr(), None, y.data_ptr(), x.numel(), drop, 0, stream) == -1
+    torch.cuda.synchronize()
+    assert all((t == 7).all() for t in (y, st, dg, db))

@@ -160,3 +160,21 @@ def test_python_entries_refuse():
     for bad in (wide.permute(0, 3, 1, 2), wide[:, :, :2], wide[:, :2], wide[..., ::2], wide[:, ::2], wide[:1, :1, :1].expand(2, 3, 4, 24)):
         with pytest.raises(ValueError, match="one stride"):
             norm._pixel_stride(bad, "x")
+
+
+@pytest.mark.parametrize("call,name,said", [(_gn, "gamma", "gamma"), (_gn, "beta", "beta"), (_gb, "gamma", "gamma"), (_gb, "beta", "beta"), (_gb, "dg", "dgamma"),
+                                            (_gb, "db", "dbeta"), (_gn, "st", "mean_rstd"), (_gb, "st", "mean_rstd")])
+def test_every_operand_that_is_no_device_memory_is_refused(call, name, said):
+    """A call's pointers are asked for one by one, the parameters and their gradients first: the first that is no memory of a GPU is named, before
+    anything is launched."""
+    host = ctypes.create_string_buffer(1 << 12)
+    p = ctypes.addressof(host) // 64 * 64 + 64
+    assert call(**{name: p}) == -1 and lib.lib().fisr_last_error(None).decode().endswith(f": {said} is not memory of a GPU")
+
+
+def test_a_counter_in_host_memory_is_refused():
+    host = (ctypes.c_uint64 * 2)()
+    p = ctypes.addressof(host)
+    assert lib.lib().fisr_train_dropout(P, None, P, 8, _drop(0.5, p), 0, None) == -1 and b"d_counter is not memory" in lib.lib().fisr_last_error(None)
+    for call in (_gn, _gb):
+        assert call(drop=_drop(0.5, p)) == -1 and b"d_counter is not memory" in lib.lib().fisr_last_error(None)
