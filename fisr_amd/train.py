@@ -45,8 +45,9 @@ class _Conv:
 class TrainNet:
     def __init__(self, weights=None, device="cuda:0", seed=2020, lambdas=None, dropout=0.0, dropout_seed=2020):
         """dropout: probability of a dropout between the two convs of every residual block while `training` is set (the reference has
-        none: 0); its masks are a function of dropout_seed, the step and the block, so a run repeats and resumes with the same ones, and
-        every rank of a data-parallel run takes a seed of its own."""
+        none: 0); its masks are a function of dropout_seed, the step and how many dropouts there were since zero_grad() or the last
+        change of the weights.  So a run repeats and resumes with the same ones, batches whose gradients are accumulated for one step
+        draw masks of their own, and every rank of a data-parallel run takes a seed of its own."""
         import torch
         if not 0.0 <= dropout < 1.0:
             raise ValueError(f"dropout = {dropout} is not in [0, 1)")
@@ -122,6 +123,7 @@ class TrainNet:
 
     def repack(self):
         """Master weights -> the conv kernel's layouts (after construction and after every Adam step)."""
+        self._dropouts = 0
         self._ck(self.L.fisr_train_pack_all(self._p(self._pack_descs), len(self.convs), self._st()))       # one launch for all 138 convs
 
     def weights_numpy(self):
@@ -166,6 +168,7 @@ class TrainNet:
         return out
 
     def zero_grad(self):
+        self._dropouts = 0
         self.gflat.zero_()
 
     def allreduce_grads(self, group=None):
@@ -216,7 +219,7 @@ class TrainNet:
         return y
 
     def next_dropout(self, p):
-        """The next norm.Dropout of this step: (dropout_seed; step and number within it)."""
+        """The next norm.Dropout of this step: (dropout_seed; step and number within it, which zero_grad() and repack() start again)."""
         from . import norm
         self._dropouts += 1
         return norm.Dropout(p, self.dropout_seed, (self.step_count << 20) + self._dropouts)
@@ -451,10 +454,9 @@ class TrainNet:
     def loss_and_grads(self, batch):
         """batch: dict of device NHWC fp32 tensors data15 [B,H,W,15], label21 [B,2H,2W,21], flow16, warp24, flow_ss2 [.,8],
         warp_ss2 [.,12].  Runs the four passes, the loss kernel per level and the whole backward.  Returns (total, terms);
-        gradients are left accumulated in the conv states (call zero_grad() first)."""
+        gradients are left accumulated in the conv states (call zero_grad() first, once for all batches of a step)."""
         torch, L = self.torch, self.L
         self.tape = []
-        self._dropouts = 0
         # The four passes share the weights, so they run as ONE pass over a batch of 4B: windows 0, 1, 2 (stride 1,
         # FISRnet.py:283-310) and the stride-2 window (:403-409) stacked along the batch axis -- a quarter of the kernel
         # launches, four times the work per launch, the same numbers (every sample is convolved independently).

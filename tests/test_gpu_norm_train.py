@@ -139,3 +139,24 @@ def test_phase_train_with_dropout(env, tmp_path):
         assert step == 1
         W.append(weights.load_weights(path, kind))
     assert sorted(W[0]) == sorted(W[1]) and any(not np.array_equal(W[0][k], W[1][k]) for k in W[0])
+
+
+def test_batches_of_one_step_draw_masks_of_their_own(env):
+    """Gradients accumulated over two batches before a step: the second batch's masks are not the first one's (the same batch twice gives
+    another loss and other gradients), and after zero_grad() or with weights packed again the numbers start where they did.  The loss' and the
+    gradients' sums are atomic: 1e-6 of the loss, and 1e-3 of the gradients' norm, which masks of their own change by far more."""
+    torch, norm, train, weights = env
+    batch = _batch(train)
+    net = train.TrainNet(weights.synthetic_weights(2020), dropout=0.2, dropout_seed=7)
+    net.zero_grad()
+    l0, _ = net.loss_and_grads(batch)
+    g0 = net.gflat.clone()
+    l1, _ = net.loss_and_grads(batch)
+    g1 = net.gflat - g0
+    assert abs(l1 - l0) > 1e-5 * l0 and float((g1 - g0).norm()) > 0.02 * float(g0.norm())
+    net.zero_grad()
+    l2, _ = net.loss_and_grads(batch)
+    assert abs(l2 - l0) <= 1e-6 * l0 and float((net.gflat - g0).norm()) < 1e-3 * float(g0.norm())
+    net.repack()
+    l3, _ = net.loss_and_grads(batch)
+    assert abs(l3 - l0) <= 1e-6 * l0
