@@ -11,6 +11,10 @@ or a range of the channels of one).  gamma, beta, statistics and their gradients
 tensors' device; workspaces come from torch's allocator, so a call can be captured into a graph.  The dropout mask is a function of
 (seed, offset, element): the backward pass is given the same numbers and nothing is stored.
 
+Autograd does not see these calls: what they return has no gradient function even where an input requires a gradient, and a program calls the
+backward functions itself (as the tape of fisr_amd/train.py does).  Tensors that a call is given to write count as changed in place: a
+graph that kept one of them for its backward pass raises there.
+
 There is no CPU fallback: without the library and a GPU every call raises.
 """
 from __future__ import annotations
@@ -144,6 +148,13 @@ def _out(x, out, cs, dev, what):
     return x.new_empty(x.shape), x.shape[3]
 
 
+def _wrote(*given):
+    """Counts the caller's tensors among `given` as changed in place."""
+    for t in given:
+        if t is not None and not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+
+
 @functools.lru_cache(4096)
 def _workspace_bytes(n, h, w, c, groups, backward):
     return _fn.ws_bytes(n, h, w, c, groups, backward)
@@ -179,6 +190,8 @@ def group_norm(x, groups, gamma=None, beta=None, *, eps=1e-5, act="none", dropou
         rc = _fn.gn(*call, ws.data_ptr(), nbytes, st)
     if rc < 0:
         _lib.check(rc)
+    if out is not None:
+        _wrote(out)
     return y, stats
 
 
@@ -191,9 +204,9 @@ def group_norm_backward(dy, x, stats, groups, gamma=None, beta=None, *, act="non
     code, dev = _type(x)
     _like(dy, x, dev, "dy")
     x_cs, dy_cs = _pixel_stride(x, "x"), _pixel_stride(dy, "dy")
-    given = dx is not None and x.numel() > 0
+    given = dx, dgamma, dbeta
     dx, dx_cs = _out(x, dx, x_cs, dev, "dx")
-    if given:
+    if given[0] is not None and x.numel():
         _apart(dx, dx_cs, dy, dy_cs, "dx")
         _apart(dx, dx_cs, x, x_cs, "dx")
     if accumulate and (dgamma is None or dbeta is None):
@@ -210,6 +223,7 @@ def group_norm_backward(dy, x, stats, groups, gamma=None, beta=None, *, act="non
                     ws.data_ptr(), nbytes, _stream(dev))
     if rc < 0:
         _lib.check(rc)
+    _wrote(*given)
     return dx, dgamma, dbeta
 
 
@@ -227,6 +241,8 @@ def dropout(x, drop, residual=None, out=None):
     rc = _fn.drop(x.data_ptr(), res, y.data_ptr(), x.numel(), _drop(drop, dev), code, _stream(dev))
     if rc < 0:
         _lib.check(rc)
+    if out is not None:
+        _wrote(out)
     return y
 
 

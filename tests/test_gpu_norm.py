@@ -412,3 +412,36 @@ def test_c_entries_refuse_host_memory_beside_device_tensors(env):
     assert L.fisr_train_dropout(x.data_ptr(), None, y.data_ptr(), x.numel(), drop, 0, stream) == -1
     torch.cuda.synchronize()
     assert all((t == 7).all() for t in (y, st, dg, db))
+
+
+def test_given_outputs_count_as_changed_in_place(env):
+    """A graph of autograd that kept a tensor which a call then writes raises in its backward pass instead of using the new values; tensors
+    that are only read do not count, nor do tensors of inference mode, which have no count."""
+    torch, norm = env
+    x, dy, gamma, beta = _inputs(torch, 2, 4, 5, 16, "f32", 9)
+    drop = norm.Dropout(0.5, 1, 2)
+    _, st = norm.group_norm(x, 4, gamma, beta)
+
+    def backward(t, **kw):
+        norm.group_norm_backward(dy, x, st, 4, gamma, beta, **{"dx": torch.empty_like(x), "dgamma": torch.empty_like(gamma), "dbeta": torch.empty_like(beta), **kw})
+
+    calls = [(x, lambda t: norm.dropout(t, drop, out=t)), (x, lambda t: norm.group_norm(t, 4, gamma, beta, out=t)), (x, lambda t: backward(t, dx=t)),
+             (gamma, lambda t: backward(t, dgamma=t)), (beta, lambda t: backward(t, dbeta=t)), (x, lambda t: norm.dropout_backward(dy, drop, out=t))]
+    for like, call in calls:
+        w = torch.ones_like(like, requires_grad=True)
+        t = w * 2
+        loss = (t * t).sum()
+        call(t)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    w = torch.ones_like(x, requires_grad=True)
+    t = w * 2
+    loss = (t * t).sum()
+    y, _ = norm.group_norm(t, 4, gamma, beta)
+    assert not y.requires_grad and not norm.dropout(t, drop, residual=t).requires_grad
+    loss.backward()
+    assert torch.equal(w.grad, torch.full_like(w, 8.0))
+    with torch.inference_mode():
+        t = x * 2
+        want, _ = norm.group_norm(t, 4, gamma, beta)
+        assert torch.equal(norm.group_norm(t, 4, gamma, beta, out=t)[0], want)
