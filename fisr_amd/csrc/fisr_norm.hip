@@ -231,19 +231,49 @@ const char* drop_error(const fisr_dropout* d, DropArgs& out) {
   if ((uintptr_t)d->d_counter % 8) return "dropout: d_counter is not aligned to 8 bytes";
   return nullptr;
 }
-// The device that a call's operands are on, null ones aside; -1 where one is not memory of a GPU or of another one than those before it.  Every
-// pointer that a kernel goes to is among them: one to host memory would be a fault of the GPU.
-struct Operand { const char* name; const void* p; };
+// Where an operand lies: `count` runs of `run` bytes, `step` bytes from one to the next.
+struct Place {
+  uintptr_t at;
+  size_t run, step, count;
+  Place(const void* p, size_t bytes) : at((uintptr_t)p), run(bytes), step(bytes), count(1) {}
+  Place(const void* p, size_t pixels, size_t c, size_t cs, size_t elem_bytes) : at((uintptr_t)p), run(c * elem_bytes), step(cs * elem_bytes), count(pixels) {
+    if (run == step || count == 1) { run *= count; step = run; count = 1; }      // no gaps
+  }
+  uintptr_t end() const { return at + (count - 1) * step + run; }
+  bool same(const Place& o) const { return at == o.at && run == o.run && step == o.step && count == o.count; }
+  // Whether they share a byte (runs at two steps: taken to)
+  bool meets(const Place& o) const {
+    if (!at || !o.at || !run || !o.run || end() <= o.at || o.end() <= at) return false;
+    if (count == 1 && o.count == 1) return true;
+    if (count > 1 && o.count > 1 && step != o.step) return true;
+    const size_t every = count > 1 ? step : o.step;
+    const size_t from = at >= o.at ? (at - o.at) % every : (every - (o.at - at) % every) % every;      // where a run of this begins, after one of the other's
+    const size_t run_a = std::min(run, every), run_b = std::min(o.run, every);
+    return from < run_b || from + run_a > every;
+  }
+};
+// The device that a call's operands are on, null ones aside; -1 where one is not memory of a GPU or of another one than those before it (every
+// pointer that a kernel goes to is among them: one to host memory would be a fault of the GPU), or where one that is written lies across
+// another.  IN_PLACE: read, and an OUT may be the very same.
+enum Use { READ, IN_PLACE, WRITTEN, OUT };
+struct Operand { const char* name; Use use; Place place; };
 int operands_device(std::initializer_list<Operand> operands, std::string& error) {
   int dev = -1;
   for (const Operand& o : operands) {
-    if (!o.p) continue;
-    const int d = device_of(o.p);
+    if (!o.place.at) continue;
+    const int d = device_of((const void*)o.place.at);
     if (d < 0) error = std::string(o.name) + " is not memory of a GPU";
     else if (dev >= 0 && d != dev) error = std::string(o.name) + " is memory of another GPU";
     if (!error.empty()) return -1;
     dev = d;
   }
+  for (const Operand& w : operands)
+    if (w.use >= WRITTEN)
+      for (const Operand& o : operands)
+        if (&w != &o && w.place.meets(o.place) && !(w.use == OUT && o.use == IN_PLACE && w.place.same(o.place))) {
+          error = std::string(w.name) + " overlaps " + o.name;
+          return -1;
+        }
   return dev;
 }
 size_t type_bytes(int type) { return type == FISR_TYPE_F32 ? 4 : type == FISR_TYPE_F16 || type == FISR_TYPE_BF16 ? 2 : 0; }
@@ -270,8 +300,13 @@ int norm_call(const char* who, NormArgs& a, bool backward, int n, int h, int w, 
   a.s12 = a.part + lay.part;
   a.ab = a.s12 + lay.s12;
   std::string error;
-  const int dev = operands_device({{"gamma", a.gamma}, {"beta", a.beta}, {"dgamma", a.dgamma}, {"dbeta", a.dbeta}, {"d_counter", a.drop.counter}, {"mean_rstd", mean_rstd},
-                                   {"the workspace", ws}, {"dy", a.dy}, {"x", a.x}, {backward ? "dx" : "y", a.y}}, error);
+  const size_t pixels = (size_t)n * a.p, params = (size_t)c * sizeof(float);
+  const int dev = operands_device({{"gamma", READ, {a.gamma, params}}, {"beta", READ, {a.beta, params}}, {"dgamma", WRITTEN, {a.dgamma, params}},
+                                   {"dbeta", WRITTEN, {a.dbeta, params}}, {"d_counter", READ, {a.drop.counter, sizeof(uint64_t)}},
+                                   {"mean_rstd", backward ? READ : WRITTEN, {mean_rstd, 2 * sizeof(float) * n * groups}},
+                                   {"the workspace", WRITTEN, {ws, backward || a.team < 0 ? norm_ws_bytes(a, backward) : 0}},
+                                   {"dy", IN_PLACE, {a.dy, pixels, (size_t)c, a.dycs, es}}, {"x", IN_PLACE, {a.x, pixels, (size_t)c, a.xcs, es}},
+                                   {backward ? "dx" : "y", OUT, {a.y, pixels, (size_t)c, a.ycs, es}}}, error);
   if (dev < 0) return bad(error.c_str());
   DeviceGuard guard(dev);
   NORM_HIP_OK(guard.err);
@@ -339,7 +374,8 @@ int fisr_train_dropout(const void* x, const void* residual, void* y, size_t coun
   if (!x || !y) return bad("null tensor");
   if (((uintptr_t)x | (uintptr_t)residual | (uintptr_t)y) % es) return bad("a pointer is not aligned to its element");
   std::string error;
-  const int dev = operands_device({{"d_counter", d.counter}, {"residual", residual}, {"x", x}, {"y", y}}, error);
+  const int dev = operands_device({{"d_counter", READ, {d.counter, sizeof(uint64_t)}}, {"residual", IN_PLACE, {residual, count * es}}, {"x", IN_PLACE, {x, count * es}},
+                                   {"y", OUT, {y, count * es}}}, error);
   if (dev < 0) return bad(error.c_str());
   DeviceGuard guard(dev);
   NORM_HIP_OK(guard.err);

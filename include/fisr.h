@@ -383,7 +383,9 @@ FISR_API int fisr_train_adam(float* w, const float* g, float* m, float* v, size_
  * an image and the images follow each other without gaps); `type` is the type of all of a call's tensors, the parameters, statistics
  * and parameter gradients are float32.  Arithmetic is float32 throughout, outputs are rounded once.  Results are the same bits on
  * every call (no atomics).  Nothing is kept between calls; calls that run at the same time need workspaces of their own.  Every pointer
- * of a call, the parameters' and the counter's too, has to be memory of the output's device: FISR_EINVAL otherwise, and nothing is launched. */
+ * of a call, the parameters' and the counter's too, has to be memory of the output's device: FISR_EINVAL otherwise, and nothing is launched; so
+ * too where something that is written overlaps another operand without being it where that is allowed (other channels of the same pixels
+ * are no overlap). */
 enum { FISR_TYPE_F32 = 0, FISR_TYPE_F16 = 1, FISR_TYPE_BF16 = 2 };
 enum { FISR_ACT_NONE = 0, FISR_ACT_RELU = 1, FISR_ACT_SILU = 2, FISR_ACT_GELU = 3 /* z * Phi(z) */ };
 /* Dropout whose mask is a function of (seed, offset, element) and is never stored: element i of the dense tensor [n,h,w,c] is dropped

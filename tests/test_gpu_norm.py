@@ -445,3 +445,63 @@ def test_given_outputs_count_as_changed_in_place(env):
         t = x * 2
         want, _ = norm.group_norm(t, 4, gamma, beta)
         assert torch.equal(norm.group_norm(t, 4, gamma, beta, out=t)[0], want)
+
+
+def test_c_entries_refuse_outputs_across_other_operands(env):
+    """What a call writes is apart from all else that it goes to, but where the very same tensor is allowed and beside other channels of the same
+    pixels.  Refused calls launch nothing."""
+    import ctypes
+    from fisr_amd import lib
+    torch, norm = env
+    L = lib.lib()
+    n, h, w, c, g = 2, 40, 50, 64, 4
+    need = L.fisr_train_groupnorm_workspace_bytes(n, h, w, c, g, 1)
+    count = n * h * w * c
+    buf = torch.full((16 * count,), 7.0, device="cuda:0")
+    f = {"x": 0, "dy": 2 * count, "y": 4 * count, "gamma": 8 * count, "beta": 8 * count + c, "dgamma": 8 * count + 2 * c, "dbeta": 8 * count + 3 * c,
+         "st": 8 * count + 4 * c, "counter": 8 * count + 5 * c, "ws": 9 * count}
+    assert 16 < need <= 4 * 7 * count
+    buf[f["counter"]:f["counter"] + 2] = 0
+    stream = torch.cuda.current_stream().cuda_stream
+
+    def call(backward, cs=None, **at):
+        p = {k: buf.data_ptr() + 4 * v for k, v in {**f, **at}.items()}
+        cs = {"x": c, "dy": c, "y": c, **(cs or {})}
+        drop = ctypes.byref(lib.DropoutDesc(0.5, 1, 2, p["counter"]))
+        if backward:
+            rc = L.fisr_train_groupnorm_bwd(p["x"], cs["x"], p["dy"], cs["dy"], p["gamma"], p["beta"], p["st"], p["y"], cs["y"], p["dgamma"], p["dbeta"], 0, n, h, w, c,
+                                            g, 0, drop, 0, p["ws"], need, stream)
+        else:
+            rc = L.fisr_train_groupnorm(p["x"], cs["x"], p["gamma"], p["beta"], p["y"], cs["y"], p["st"], n, h, w, c, g, 1e-5, 0, drop, 0, p["ws"], need, stream)
+        return rc, L.fisr_last_error(None).decode()
+
+    small = 2 * c                                           # pixels 2 c apart: room for another tensor's channels
+    for backward, what, kw in [
+            (False, "y overlaps x", dict(y=4)), (False, "y overlaps x", dict(y=count - 4)), (False, "y overlaps gamma", dict(gamma=4 * count + 8)),
+            (False, "y overlaps beta", dict(beta=5 * count - 4)), (False, "mean_rstd overlaps x", dict(st=8)), (False, "mean_rstd overlaps gamma", dict(st=8 * count)),
+            (False, "d_counter", dict(counter=4 * count)), (False, "the workspace overlaps x", dict(ws=count - 4)), (False, "the workspace overlaps y", dict(ws=4 * count)),
+            (False, "y overlaps x", dict(y=c - 4, cs=dict(x=small, y=small))), (False, "y overlaps x", dict(y=0, cs=dict(x=small))),
+            (True, "dx overlaps x", dict(y=4)), (True, "dx overlaps dy", dict(y=2 * count + 4)), (True, "dgamma overlaps gamma", dict(dgamma=8 * count)),
+            (True, "dgamma overlaps dbeta", dict(dbeta=8 * count + 2 * c)), (True, "dgamma overlaps dbeta", dict(dbeta=8 * count + c + 4)),
+            (True, "mean_rstd", dict(dgamma=8 * count + 4 * c)), (True, "dgamma overlaps x", dict(dgamma=4)), (True, "the workspace overlaps dx", dict(ws=5 * count - 4)),
+            (True, "overlaps the workspace", dict(ws=8 * count - 4))]:
+        rc, said = call(backward, **kw)
+        assert rc == -1 and what in said, (what, kw, rc, said)
+    d = ctypes.byref(lib.DropoutDesc(0.5, 1, 2, None))
+    at = buf.data_ptr()
+    for res, y, what in ((None, 4, "y overlaps x"), (8 * count, 8 * count - 4, "y overlaps residual"), (8 * count, 4 * (count - 1), "y overlaps x")):
+        assert L.fisr_train_dropout(at, None if res is None else at + res, at + y, count, d, 0, stream) == -1 and what in L.fisr_last_error(None).decode()
+    torch.cuda.synchronize()
+    untouched = buf.clone()
+    untouched[f["counter"]:f["counter"] + 2] = 7.0
+    assert (untouched == 7).all()
+    # allowed: in place, other channels of the same pixels, neighbours without a gap
+    for backward, kw in [(False, dict(y=0)), (False, dict(y=c, cs=dict(x=small, y=small))), (False, dict(y=count)), (True, dict(y=0)), (True, dict(y=2 * count)),
+                         (True, dict(y=3 * count)), (True, dict(dy=c, cs=dict(x=small, dy=small)))]:
+        rc, said = call(backward, **kw)
+        assert rc == 0, (kw, said)
+    torch.cuda.synchronize()
+    x, dy, gamma, beta = _inputs(torch, 1, 4, 4, 16, "f32", 1)
+    _, st = norm.group_norm(x, 4, gamma, beta)
+    with pytest.raises(lib.FisrError, match="dgamma overlaps gamma"):
+        norm.group_norm_backward(dy, x, st, 4, gamma, beta, dgamma=gamma)
