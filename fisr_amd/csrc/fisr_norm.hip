@@ -187,7 +187,7 @@ template <typename T, int V> void launch_any(NormArgs a, bool backward, hipStrea
   a.cb = (cv + ny - 1) / ny;
   a.rows = 256 / a.cb;
   const dim3 grid(a.n * a.chunks, ny), joins(a.n * a.groups);
-  const bool wide = a.chunks * a.d > JOIN_WIDE;
+  const bool wide = a.chunks * a.d > JOIN_WIDE && joins.x <= 0xffffffffu / 1024;         // (a grid holds less than 2^32 threads)
   if (!backward) {
     hipLaunchKernelGGL((norm_stats_kernel<T, V>), grid, dim3(256), 0, st, a);
     if (wide) hipLaunchKernelGGL(norm_stats_join_kernel<1024>, joins, dim3(1024), 0, st, a);

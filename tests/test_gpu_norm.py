@@ -505,3 +505,27 @@ def test_c_entries_refuse_outputs_across_other_operands(env):
     _, st = norm.group_norm(x, 4, gamma, beta)
     with pytest.raises(lib.FisrError, match="dgamma overlaps gamma"):
         norm.group_norm_backward(dy, x, st, 4, gamma, beta, dgamma=gamma)
+
+
+def test_the_most_groups_with_wide_joins(env):
+    """n * groups = 2^22, the limit, in groups of more channels than a join of 256 threads is meant for: a launch of 1024 threads a group would be
+    2^32, one more than a grid holds.  One pixel an image, all images alike but the last.  A group is 4097 values: bounds as above with K for 4096 values in
+    float64 joins of single values (no chain of float32 sums: E each), so y is off by a few E before it is rounded."""
+    torch, norm = env
+    torch.cuda.empty_cache()
+    n, c, groups = 1 << 20, 16388, 4
+    if torch.cuda.mem_get_info()[0] < 185 << 30:
+        pytest.skip("needs 185 GB of device memory")
+    r = np.random.default_rng(1)
+    rows = r.standard_normal((2, c)) * (0.5 + r.random(c)) + 0.5
+    rows = _to(torch, rows, "bf16")
+    x = rows[0].expand(n, 1, 1, c).contiguous()
+    x[-1, 0, 0] = rows[1]
+    _, st = norm.group_norm(x, groups, out=x)
+    for i, row in ((0, 0), (1, 0), (n // 2, 0), (n - 2, 0), (n - 1, 1)):
+        want, mean, rstd, _, _ = no.forward(_np(rows[row]).reshape(1, 1, 1, c), groups, 1.0, 0.0, 1e-5, "none")
+        assert np.abs(_np(st[0, i]) - mean[0]).max() <= 4 * E and np.abs(_np(st[1, i]) / rstd[0] - 1).max() <= 8 * E
+        _within(_np(x[i, 0, 0]), want[0, 0, 0], 2.0 ** -8 * np.abs(want[0, 0, 0]) + 16 * E * (1 + np.abs(want[0, 0, 0])), i)
+    assert (st[:, :-1] == st[:, :1]).all()
+    del x, st
+    torch.cuda.empty_cache()
