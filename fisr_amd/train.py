@@ -232,8 +232,9 @@ class TrainNet:
         return y
 
     def group_norm(self, x, groups, gamma, beta, ggamma, gbeta, eps=1e-5, act="none", drop=None):
-        """norm.group_norm, recorded: drop(act(gn(x) * gamma + beta)); backward() adds the parameters' gradients to ggamma and gbeta, as
-        the convs' do (four passes share the weights)."""
+        """norm.group_norm, recorded: drop(act(gn(x) * gamma + beta)); backward() adds the parameters' gradients to ggamma and gbeta
+        (None: not wanted), as the convs' do (four passes share the weights).  These tensors are the caller's: zero_grad(), allreduce_grads(),
+        adam_step() and the checkpoints go over the convs alone."""
         from . import norm
         y, stats = norm.group_norm(x, groups, gamma, beta, eps=eps, act=act, dropout=drop)
         self.tape.append(("norm", x, stats, groups, gamma, beta, ggamma, gbeta, act, drop, y))
@@ -401,6 +402,7 @@ class TrainNet:
                 g = grads.pop(y.data_ptr(), None)
                 if g is None:
                     continue
+                ggamma, gbeta = (self.zeros(x.shape[3]) if t is None else t for t in (ggamma, gbeta))
                 dx, _, _ = norm.group_norm_backward(g, x, stats, groups, gamma, beta, act=act, dropout=drop, dgamma=ggamma, dbeta=gbeta,
                                                     accumulate=True)
                 self._acc(grads, x, dx)

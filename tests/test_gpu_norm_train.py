@@ -160,3 +160,23 @@ def test_batches_of_one_step_draw_masks_of_their_own(env):
     net.repack()
     l3, _ = net.loss_and_grads(batch)
     assert abs(l3 - l0) <= 1e-6 * l0
+
+
+def test_normalisation_on_the_tape_without_parameters(env):
+    """No gamma and beta, or gradients of one that are not wanted: dx is that of ones and zeros, and the wanted gradient is what it was."""
+    torch, norm, train, weights = env
+    net = train.TrainNet(weights.synthetic_weights(3))
+    r = np.random.default_rng(5)
+    x, gy = (torch.from_numpy(r.standard_normal((2, 7, 9, 64)).astype(np.float32)).cuda() for _ in range(2))
+    one, zero = torch.ones(64, device="cuda"), torch.zeros(64, device="cuda")
+    got = []
+    acc = net._acc
+    net._acc = lambda grads, t, g: (got.append(g.clone()), acc(grads, t, g))
+    for gamma, beta, wants in ((one, zero, (1, 1)), (None, None, (0, 0)), (one, zero, (1, 0)), (one, zero, (0, 1))):
+        grads = [torch.zeros(64, device="cuda") if k else None for k in wants]
+        y = net.group_norm(x, 8, gamma, beta, *grads, act="silu")
+        net.backward([(y, gy)])
+        if wants == (1, 1):
+            want = grads
+        assert torch.equal(got[-1], got[0]) and all(g is None or torch.equal(g, w) for g, w in zip(grads, want))
+    assert len(got) == 4
