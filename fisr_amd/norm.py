@@ -160,7 +160,7 @@ def _workspace_bytes(n, h, w, c, groups, backward):
     return _fn.ws_bytes(n, h, w, c, groups, backward)
 
 
-_several = set()          # shapes whose forward call has asked for a workspace: one launch does not hold them
+_several = set()          # calls' shapes, strides and alignments that have asked for a workspace: one launch does not hold them
 
 
 def group_norm(x, groups, gamma=None, beta=None, *, eps=1e-5, act="none", dropout=None, out=None):
@@ -179,7 +179,7 @@ def group_norm(x, groups, gamma=None, beta=None, *, eps=1e-5, act="none", dropou
     call = (x.data_ptr(), x_cs, _param(gamma, dev, (c,), "gamma"), _param(beta, dev, (c,), "beta"), y.data_ptr(), y_cs, stats.data_ptr(), n, h, w, c, groups,
             eps, _act(act), _drop(dropout, dev), code)
     st = _stream(dev)
-    key = (shape, groups, code)
+    key = (shape, groups, code, x_cs, y_cs, (call[0] | call[4]) & 15)
     rc = _ENOMEM if key in _several else _fn.gn(*call, None, 0, st)
     if rc == _ENOMEM:
         if len(_several) >= 4096:

@@ -529,3 +529,21 @@ def test_the_most_groups_with_wide_joins(env):
     assert (st[:, :-1] == st[:, :1]).all()
     del x, st
     torch.cuda.empty_cache()
+
+
+def test_an_unaligned_call_leaves_the_aligned_ones_as_they_were(env):
+    """3 x 3 pixels of 1024 float16 channels in one group: one launch and no workspace where vectors of 16 bytes are possible, several launches from an
+    address that allows none.  After such a call the aligned one still allocates y and the statistics alone."""
+    torch, norm = env
+    x, _, gamma, beta = _inputs(torch, 2, 3, 3, 1024, "f16", 6)
+    odd = torch.empty(x.numel() + 8, dtype=x.dtype, device="cuda:0")[1:1 + x.numel()].view(x.shape)
+    odd.copy_(x)
+
+    def allocations(t):
+        before = torch.cuda.memory_stats()["allocation.all.allocated"]
+        kept = norm.group_norm(t, 1, gamma, beta)
+        return torch.cuda.memory_stats()["allocation.all.allocated"] - before, kept
+
+    allocations(x)
+    allocations(odd)
+    assert allocations(odd)[0] == 3 and allocations(x)[0] == 2
