@@ -180,3 +180,38 @@ def test_normalisation_on_the_tape_without_parameters(env):
             want = grads
         assert torch.equal(got[-1], got[0]) and all(g is None or torch.equal(g, w) for g, w in zip(grads, want))
     assert len(got) == 4
+
+
+def test_the_command_drops_in_training_and_not_in_validation(env, tmp_path, monkeypatch):
+    """--dropout P is the P of the network that the command trains: each of its training passes has a dropout in every residual block, its
+    validation passes have none, and without the option there is none at all."""
+    torch, norm, train, weights = env
+    from fisr_amd import main
+    nets = []
+
+    class Seen(train.TrainNet):
+        def __init__(self, *a, **kw):
+            super().__init__(*a, **kw)
+            self.passes = []                                    # (training, dropouts)
+            nets.append(self)
+
+        def model(self, x):
+            self.passes.append([self.training, 0])
+            return super().model(x)
+
+        def dropout(self, x, drop, residual=None):
+            assert drop.p == 0.2 and residual is None
+            self.passes[-1][1] += 1
+            return super().dropout(x, drop, residual)
+
+    monkeypatch.setattr(train, "TrainNet", Seen)
+    blocks = sum(name.endswith("/conv/1") and "res_block" in name for name, _, _ in weights.conv_specs())
+    assert blocks > 10
+    for k, extra in enumerate((["--dropout", "0.2"], [])):
+        d = str(tmp_path / str(k))
+        assert main.main(["--phase", "train", "--synthetic_train", "4", "--epoch", "1", "--batch_size", "2", "--val_data_size", "2", "--val_batch_size", "2",
+                          "--lr_type", "no_decay", "--checkpoint_dir", d + "/ck", "--text_dir", d + "/tx", "--log_dir", d + "/lg", "--test_img_dir", d + "/ti"] + extra) == 0
+    assert [n.dropout_p for n in nets] == [0.2, 0.0]
+    for net, drops in zip(nets, (blocks, 0)):
+        assert {t for t, _ in net.passes} == {True, False}
+        assert all(n == (drops if training else 0) for training, n in net.passes), net.passes
