@@ -90,15 +90,18 @@ def build(force: bool = False, verbose: bool = False, diag: bool = False, define
     flags = [hipcc_path(), "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden"] + \
             (["-DFISR_DIAG"] if diag else []) + [f"-D{x}" for x in defines]
     with tempfile.TemporaryDirectory() as d:
-        # fisr_api.hip's Winograd kernels write packed float32 instructions by hand; everything else is compiled without them
-        norm_o = os.path.join(d, "fisr_norm.o")
-        norm = flags + ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-c", "-o", norm_o, os.path.join(CSRC, "fisr_norm.hip")]
-        cmd = flags + ["-shared", "-Wl,--version-script=" + os.path.join(CSRC, "exports.map"),
-                       f'-DFISR_SRC_HASH="{source_hash()}"', "-o", target, os.path.join(CSRC, "fisr_api.hip"), "-x", "none", norm_o]
+        # fisr_norm.hip is compiled without packed float32 instructions; fisr_api.hip is not: its Winograd kernels write them by hand
+        units = {"fisr_api": [f'-DFISR_SRC_HASH="{source_hash()}"'], "fisr_norm": ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]}
+        objects = [os.path.join(d, u + ".o") for u in units]
+        cmds = [flags + extra + ["-c", "-o", o, os.path.join(CSRC, u + ".hip")] for (u, extra), o in zip(units.items(), objects)]
+        link = flags + ["-shared", "-Wl,--version-script=" + os.path.join(CSRC, "exports.map"), "-o", target] + objects
         if verbose:
-            print(" ".join(norm), " ".join(cmd), sep="\n")
-        subprocess.check_call(norm)
-        subprocess.check_call(cmd)
+            print(*(" ".join(c) for c in cmds + [link]), sep="\n")
+        running = [subprocess.Popen(c) for c in cmds]
+        failed = [subprocess.CalledProcessError(p.returncode, c) for p, c in zip(running, cmds) if p.wait()]
+        if failed:
+            raise failed[0]
+        subprocess.check_call(link)
     return target
 
 

@@ -178,3 +178,12 @@ def test_a_counter_in_host_memory_is_refused():
     assert lib.lib().fisr_train_dropout(P, None, P, 8, _drop(0.5, p), 0, None) == -1 and b"d_counter is not memory" in lib.lib().fisr_last_error(None)
     for call in (_gn, _gb):
         assert call(drop=_drop(0.5, p)) == -1 and b"d_counter is not memory" in lib.lib().fisr_last_error(None)
+
+
+def test_the_build_entry_compiles_what_is_built_already(monkeypatch):
+    """build() is what says that the sources compile, so it compiles them where a library is there too."""
+    import __graft_entry__ as entry
+    calls = []
+    monkeypatch.setattr(lib, "build", lambda force=False, verbose=False: (calls.append(force), lib.SO_PATH)[1])
+    entry.build()
+    assert calls == [True]
