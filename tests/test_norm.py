@@ -180,6 +180,22 @@ def test_a_counter_in_host_memory_is_refused():
         assert call(drop=_drop(0.5, p)) == -1 and b"d_counter is not memory" in lib.lib().fisr_last_error(None)
 
 
+def test_strides_and_places_exactly():
+    """The stride of a single pixel's channels is their number, whatever buffer they are a range of; ranges of channels before x, behind it and
+    across it."""
+    import torch
+    from fisr_amd import norm
+    wide = torch.zeros(2, 3, 4, 24)
+    assert norm._pixel_stride(wide[:1, :1, :1, 4:8], "x") == 4
+    x = wide[..., 12:20]
+    for ok in (wide[..., 0:8], wide[..., 4:12], x):
+        assert ok.shape == x.shape
+        norm._apart(ok, 24, x, 24, "out")
+    for bad in (wide[..., 5:13], wide[..., 13:21], wide[..., 16:24]):
+        with pytest.raises(ValueError, match="overlaps"):
+            norm._apart(bad, 24, x, 24, "out")
+
+
 def test_the_build_entry_compiles_what_is_built_already(monkeypatch):
     """build() is what says that the sources compile, so it compiles them where a library is there too."""
     import __graft_entry__ as entry
