@@ -547,3 +547,170 @@ def test_an_unaligned_call_leaves_the_aligned_ones_as_they_were(env):
     allocations(x)
     allocations(odd)
     assert allocations(odd)[0] == 3 and allocations(x)[0] == 2
+
+
+# ---- what full-size calls take: float64 on the GPU, an image at a time, with the bounds of the first docstring ----
+def _act64(torch, z, act):
+    """act'(z) and the bound on its curvature."""
+    if act == "silu":
+        sg = torch.sigmoid(z)
+        return sg * (1 + z * (1 - sg)), 1.0
+    if act == "gelu":
+        return torch.special.ndtr(z) + z * torch.exp(-0.5 * z * z) * 0.3989422804014327, 1.0
+    return torch.ones_like(z), 0.0
+
+
+def _check_backward(torch, x, dy, mask, stats, got, groups, gamma, beta, act, t, k, slices=1):
+    """dx, dgamma, dbeta of group_norm_backward(dy, x, stats ...); mask: what multiplies dy.  k: a thread's chain and the joins (K of the first
+    docstring).  Images are worked on in `slices` ranges of pixels."""
+    dx, dg, db = got
+    n, c = x.shape[0], x.shape[3]
+    p, d = x[0].numel() // c, c // groups
+    g, b = gamma.double(), beta.double()
+    bounds = list(range(0, p, (p + slices - 1) // slices)) + [p]
+    parts = [slice(lo, hi) for lo, hi in zip(bounds, bounds[1:])]
+    sums = torch.zeros(4, c, dtype=torch.float64, device=x.device)              # dgamma, its bound, dbeta, its bound
+    chan = lambda v: v.repeat_interleave(d)  # noqa: E731
+    for i in range(n):
+        xi, dyi, mi, dxi = (v[i].view(p, c) for v in (x, dy, mask, dx))
+        far = max(float(xi[q].abs().max()) for q in parts)
+        mean = sum(xi[q].double().sum(0) for q in parts).view(groups, d).sum(1) / (p * d)
+        var = sum(((xi[q].double() - chan(mean)) ** 2).sum(0) for q in parts).view(groups, d).sum(1) / (p * d)
+        rstd = 1 / torch.sqrt(var + 1e-5)
+        emean, erstd = torch.full_like(mean, k * E * far), (k + 2 * far * rstd) * E
+        assert ((stats[0, i].double() - mean).abs() <= emean + E * mean.abs()).all() and ((stats[1, i].double() - rstd).abs() <= (erstd + E) * rstd).all()
+        mean, rstd, emean, erstd = map(chan, (mean, rstd, emean, erstd))
+
+        def terms(q):
+            xh = (xi[q].double() - mean) * rstd
+            exh = rstd * emean + xh.abs() * (erstd + 4 * E)
+            z = xh * g + b
+            ez = g.abs() * exh + E * z.abs()
+            slope, curve = _act64(torch, z, act)
+            dyq = dyi[q].double() * mi[q].double()
+            dz = dyq * slope
+            edz = dyq.abs() * (curve * ez + 1e-6)
+            ta = edz + k * E * dz.abs()
+            return xh, exh, dz, edz, ta, ta * xh.abs() + dz.abs() * exh
+
+        acc = torch.zeros(6, c, dtype=torch.float64, device=x.device)           # sums of dz, dz xh, their terms' bounds, |dz|, |dz xh|
+        for q in parts:
+            xh, exh, dz, edz, ta, tb = terms(q)
+            acc += torch.stack([v.sum(0) for v in (dz, dz * xh, ta, tb, dz.abs(), (dz * xh).abs())])
+            del xh, exh, dz, edz, ta, tb
+        sums += torch.stack((acc[1], acc[3], acc[0], acc[2]))
+        grp = lambda v, w: chan((v * w).view(groups, d).sum(1) / (p * d))  # noqa: E731
+        s1, s2 = grp(acc[0], g), grp(acc[1], g)
+        ga, gb, m1, m2 = (grp(v, g.abs()) for v in acc[2:])
+        for q in parts:
+            xh, exh, dz, edz, _, _ = terms(q)
+            want = rstd * (dz * g - s1 - xh * s2)
+            bound = rstd * (g.abs() * (edz + 8 * E * dz.abs()) + ga + xh.abs() * gb + exh * m2 + 8 * E * (m1 + xh.abs() * m2)) + HALF[t] * want.abs() + TINY[t]
+            bound += erstd * (want.abs() + rstd * (g.abs() * dz.abs() + m1 + xh.abs() * m2))
+            off = (dxi[q].double() - want).abs() - bound
+            assert float(off.max()) <= 0, (i, q, float(off.max()))
+            del xh, exh, dz, edz, want, bound, off
+    assert ((dg.double() - sums[0]).abs() <= sums[1] + E * sums[0].abs()).all()
+    assert ((db.double() - sums[2]).abs() <= sums[3] + E * sums[2].abs()).all()
+
+
+def _large(torch, n, h, w, c, t, seed):
+    gen = torch.Generator(device="cuda:0").manual_seed(seed)
+    normal = lambda *shape: torch.randn(*shape, generator=gen, device="cuda:0")  # noqa: E731
+    x, dy = (torch.empty(n, h, w, c, dtype=_type(torch, t), device="cuda:0") for _ in range(2))
+    scale, shift = 0.5 + normal(c).abs().clamp(max=1), 0.5 + normal(c)
+    for i in range(n):
+        x[i] = (normal(h, w, c) * scale + shift).to(x.dtype)
+        dy[i] = normal(h, w, c).to(x.dtype)
+    return x, dy, 1 + 0.2 * normal(c), 0.2 * normal(c)
+
+
+@pytest.mark.parametrize("t,n,h,w,c,groups,act,p", [
+    ("bf16", 4, 544, 992, 64, 8, "silu", 0.1),               # 552 MB of x and dy: reads past the caches, pieces by size
+    ("f32", 2, 544, 992, 64, 16, "gelu", 0.25),              # the same in float32, where a generator block is two threads' work
+    ("f16", 1, 544, 992, 128, 32, "gelu", 0.0),              # 276 MB, one image: the join between the launches
+    ("f32", 32, 116, 116, 64, 8, "none", 0.1),               # 220 MB: pieces by size, through the caches
+    ("bf16", 5, 400, 300, 72, 9, "silu", 0.1),               # 173 MB: 1536 pieces
+])
+def test_large_backward(env, t, n, h, w, c, groups, act, p):
+    """Chains: at most 132 values a thread, 256 a join."""
+    torch, norm = env
+    x, dy, gamma, beta = _large(torch, n, h, w, c, t, 7)
+    drop = norm.Dropout(p, 91, 1 << 35)
+    mask = norm.dropout(torch.ones(x.shape, device="cuda:0"), drop)
+    _, st = norm.group_norm(x, groups, gamma, beta, act=act, dropout=drop)
+    got = norm.group_norm_backward(dy, x, st, groups, gamma, beta, act=act, dropout=drop)
+    _check_backward(torch, x, dy, mask, st, got, groups, gamma, beta, act, t, K + 132)
+
+
+def test_backward_past_32_bits(env):
+    """4.3e9 elements, dx in dy's place.  A thread's chain in the sums is 131762 pixels of a chunk / 32 rows = 4118; K follows it."""
+    torch, norm = env
+    torch.cuda.empty_cache()
+    n, h, w, c, groups = 3, 4731, 4733, 64, 4
+    x, dy, gamma, beta = _large(torch, n, h, w, c, "bf16", 8)
+    assert x.numel() > 1 << 32
+    drop = norm.Dropout(0.25, 5, 6)
+    mask = norm.dropout(torch.ones_like(x), drop)             # 4 / 3 in bfloat16: 1.3359, a factor of its own
+    for first in (0, (1 << 32) - 512, x.numel() - 1024):
+        want = no.drop_factor((1024,), 0.25, 5, 6, first)
+        assert np.array_equal(_np(mask.view(-1)[first:first + 1024]) > 0, want > 0)
+    _, st = norm.group_norm(x, groups, gamma, beta, act="silu", dropout=drop)
+    dx = dy.clone()
+    got = norm.group_norm_backward(dx, x, st, groups, gamma, beta, act="silu", dropout=drop, dx=dx)
+    mask.clamp_(max=1.0)
+    dy_scaled = 65536 / (65536 - 16384)
+    _check_backward(torch, x, dy, _Times(mask, dy_scaled), st, got, groups, gamma, beta, "silu", "bf16", 4118 + K, slices=8)
+    del x, dy, mask, dx, got
+    torch.cuda.empty_cache()
+
+
+class _Times:
+    """A mask of ones and zeros times a factor that its type does not hold."""
+
+    def __init__(self, mask, factor):
+        self.mask, self.factor = mask, factor
+
+    def __getitem__(self, i):
+        return _Times(self.mask[i], self.factor)
+
+    def view(self, *shape):
+        return _Times(self.mask.view(*shape), self.factor)
+
+    def double(self):
+        return self.mask.double() * self.factor
+
+
+@pytest.mark.parametrize("t,count", [("f32", 22000003), ("f16", 44000005), ("bf16", 44000000)])
+def test_large_dropout_with_residual(env, t, count):
+    """More than 160 MB of reads, which go past the caches; the tail of the odd counts too."""
+    torch, norm = env
+    gen = torch.Generator(device="cuda:0").manual_seed(4)
+    x, res = (torch.randn(count, generator=gen, device="cuda:0").to(_type(torch, t)) for _ in range(2))
+    fac = torch.from_numpy(no.drop_factor((count,), 0.3, 61, 62)).cuda()
+    got = norm.dropout(x, norm.Dropout(0.3, 61, 62), residual=res)
+    kept = x.double() * fac
+    want = kept + res.double()
+    assert ((got.double() - want).abs() <= HALF[t] * want.abs() + 3 * E * (want.abs() + kept.abs()) + TINY[t]).all()
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+def test_pixels_far_apart(env, t):
+    """Channels of a buffer whose pixels are 3 M elements apart: a thread's offsets would pass 32 bits in the one-launch form, and in float32 in the
+    two-launch form too.  Against the dense call, as in test_channel_ranges_of_wider_buffers; a float32 mean goes by K E."""
+    torch, norm = env
+    x, dy, gamma, beta = _inputs(torch, 2, 2, 3, 24, t, 14)
+    wide, dwide, ywide, gwide = (torch.full((2, 2, 3, 3 << 20), 7.0, dtype=x.dtype, device="cuda:0") for _ in range(4))
+    lo, hi = (3 << 20) - 40, (3 << 20) - 16
+    wide[..., lo:hi], dwide[..., lo:hi] = x, dy
+    drop = norm.Dropout(0.3, 5, 6)
+    y0, st0 = norm.group_norm(x, 2, gamma, beta, act="gelu", dropout=drop)
+    d0 = norm.group_norm_backward(dy, x, st0, 2, gamma, beta, act="gelu", dropout=drop)
+    tol = 3 * HALF[t]
+    y1, st1 = norm.group_norm(wide[..., lo:hi], 2, gamma, beta, act="gelu", dropout=drop, out=ywide[..., lo:hi])
+    d1 = norm.group_norm_backward(dwide[..., lo:hi], wide[..., lo:hi], st1, 2, gamma, beta, act="gelu", dropout=drop, dx=gwide[..., lo:hi])
+    assert torch.allclose(st0, st1, rtol=K * E, atol=K * E) and torch.allclose(y0.double(), y1.double(), rtol=tol, atol=1e-4)
+    assert torch.allclose(d0[0].double(), d1[0].double(), rtol=tol, atol=1e-3)
+    assert all(torch.allclose(a, b, rtol=1e-4, atol=1e-4) for a, b in zip(d0[1:], d1[1:]))
+    for v in (ywide, gwide):
+        assert (v[..., :lo] == 7).all() and (v[..., hi:] == 7).all()
