@@ -82,13 +82,21 @@ int span_unit(const NormArgs& a, int v) {
 }
 
 // One launch, a span of channels of a whole image in a workgroup's registers: which variant holds it (-1: none does, or it would be slower).
+// Up to 9 vectors a thread: 48 x 48 pixels of 4 columns.  More were tried in the forward pass (bfloat16, 32 images of 128 channels in 32 groups): 12 take
+// 50 x 50 in 17.8 us against 20.6 in two launches and 55 x 55 in 19.3 against 22.6, 16 take 64 x 64 in 23.0 against 26.6 (16 images 21.6 against 19.5);
+// the backward pass holds dz as float32 beside them, 72 registers at 9 vectors of 8.
 struct TeamVariant { int threads, r; };
 constexpr TeamVariant TEAM[] = {{256, 1}, {256, 2}, {256, 4}, {256, 9}, {512, 9}};
 int team_variant(NormArgs& a, int v, int elem_bytes, bool backward) {
   const size_t elems = (size_t)a.n * a.p * a.c;
   if (elems > (size_t)env_int("NORM_TEAM_K", 16384) << 10 || wide_strides(a, 512, elem_bytes)) return -1;
   const int unit = span_unit(a, v), most = a.c / unit;
-  const int line = env_int("NORM_LINE", elems * elem_bytes > (size_t)4 << 20 ? 64 : 16);  // least bytes of a span: narrow ones read a cache line many times over
+  // Least bytes of a span.  Narrow ones read a cache line many times over (32 x 24 x 24 x 256 bfloat16 in 64 groups, 9.4 MB: 11.9 us at 64 bytes, 12.5 at 16,
+  // 13.8 at 128; backward 15.5, 16.1, 18.6), small tensors want the workgroups more (8 x 24 x 24 x 256 in 64 groups, 2.4 MB: 9.0 at 16, 10.9 at 64; but with
+  // 32 images of 12 x 12 8.6 and 7.7).  Whole lines of 128 bytes where there are 512 workgroups all the same: 128 x 8 x 8 x 512 bfloat16 in 64 groups 11.7 us
+  // against 14.3, backward 14.9 against 19.8; 64 x 16 x 16 x 512 in 32 groups 15.5 against 14.2; without the limit of 512 16 x 24 x 24 x 512 in 32 groups takes
+  // 13.7 instead of 11.8, backward 16.7 instead of 15.1.
+  const int line = env_int("NORM_LINE", elems * elem_bytes > (size_t)4 << 20 ? 64 : 16);
   int best = -1, best_span = 0;
   for (int k = 1; k <= most; ++k) {
     const int span = k * unit, cols = span / v;
@@ -129,7 +137,9 @@ bool two_tiling(NormArgs& a, int v, int elem_bytes, bool backward) {
   const int unit = span_unit(a, v), most = a.c / unit;
   int k = std::min(most, 256 * v / unit);
   while (k > 0 && most % k) --k;
-  // (no such span, or one of few columns with more channels beside it: workgroups of any channels read whole lines)
+  // (no such span, or one of few columns with more channels beside it: workgroups of any channels read whole lines.  About 4 M elements of 4 images, by
+  // columns x spans, this form against that one: 3 x 347 float32 1274 and 49 us, 17 x 61 237 and 48, 41 x 31 137 and 57; 67 x 17 75 and 52, 113 x 11 53 and 59,
+  // 100 x 5 42 and 72, 127 x 3 38 and 72; backward 67 x 17 138 and 80, 113 x 11 107 and 82, 100 x 5 84 and 90, 127 x 3 68 and 88)
   if (k == 0 || (k < most && k * unit / v < 64)) return false;
   set_team(a, v, 256, k * unit);
   // First launch: two long-lived workgroups a CU, whose numbers have to be joined.  Second: four a CU, six above 48 MB (272 x 496 x 128 bfloat16,
@@ -326,8 +336,9 @@ template <typename T> int launch_dropout(const T* x, const T* res, T* y, size_t 
   const size_t per = (size_t)256 * (16 / sizeof(T)) * DROP_U, grid = (count + per - 1) / per, bytes = count * sizeof(T);
   if (grid >= 1u << 24) return -1;
   const dim3 g((unsigned)grid), b(256);
-  // all accesses past the caches beyond 160 MB of reads (202 MB: 64 us against 74 plain; 75 MB: 25.6 against 24.7); the writes alone where
-  // there is no residual and they pass the L2 caches (75 MB: 23.0 against 24.7; with a residual 38.4 against 35.4)
+  // all accesses past the caches beyond 160 MB of reads (float32, 202 MB: 64 us against 74 plain; two inputs of 132 MB 62 against 71, of 94 MB 44.5 against
+  // 43.9, of 75 MB 35.9 against 35.3); the writes alone where there is no residual and they pass the L2 caches (75 MB: 22.8 against 24.9; 38 MB 12.3
+  // against 12.1, 94 MB 29.4 against 29.8, 132 MB 43.5 against 39.7; with a residual 35.4 against 35.3)
   if (bytes * (res ? 2 : 1) > (size_t)160 << 20) hipLaunchKernelGGL((dropout_kernel<T, true, true>), g, b, 0, st, x, res, y, count, d);
   else if (!res && bytes > (size_t)32 << 20) hipLaunchKernelGGL((dropout_kernel<T, false, true>), g, b, 0, st, x, res, y, count, d);
   else hipLaunchKernelGGL((dropout_kernel<T, false, false>), g, b, 0, st, x, res, y, count, d);

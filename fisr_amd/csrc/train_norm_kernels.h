@@ -508,9 +508,11 @@ template <typename T, int V, int U> __device__ __forceinline__ void stats_batch(
   for (int e = 0; e < V; ++e) { const float dm = bm[e] - mean[e]; mean[e] += dm * w; m2[e] += b2[e] + dm * dm * nw; }
 }
 
-// The vectors of a thread in a chunk, U at a time, the next ones on their way while these are worked on: two buffers in turn (a copy between
+// The vectors of a thread in a chunk, U at a time, the next ones asked for before these are worked on: two buffers in turn (a copy between
 // them would cost as many instructions as a vector's arithmetic).  `load(buffer, r, m)` and `work(buffer, r, m)` take vectors r .. r + m - 1;
-// m is U but for the last ones.  fetch() loads the first, finish() does the rest.
+// m is U but for the last ones.  fetch() loads the first, finish() does the rest.  As compiled, every other fetch alone is still on its way
+// during the work: a whole batch and the last one fill the same buffer on paths that join, after which the number of loads under way is not
+// known, and the wait before the work is for all of them.
 template <int U, typename B> struct Chunk {
   int full, tail;
   B b0, b1;

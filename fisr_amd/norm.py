@@ -165,7 +165,8 @@ _several = set()          # calls' shapes, strides and alignments that have aske
 
 def group_norm(x, groups, gamma=None, beta=None, *, eps=1e-5, act="none", dropout=None, out=None):
     """drop(act((x - mean) * rstd * gamma + beta)) with the mean and rstd = 1 / sqrt(var + eps) of every image's groups of channels.
-    Returns (y, stats), stats [2, N, groups] float32: means and rstd, what group_norm_backward takes.  `out` may be x."""
+    Returns (y, stats), stats [2, N, groups] float32: means and rstd, what group_norm_backward takes.  `out` may be x.  var + eps has to
+    be at least 2^-126."""
     n, h, w, c = shape = _images(x, groups)
     code, dev = _type(x)
     if out is None and x.is_contiguous():

@@ -401,7 +401,8 @@ typedef struct fisr_dropout {
 } fisr_dropout;
 /* y = drop(act((x - mean) * rstd * gamma + beta)), mean and rstd = 1 / sqrt(var + eps) over the pixels and the c / groups channels of
  * a group.  gamma, beta [c] (nullable: ones, zeros); mean_rstd [2][n][groups]: means, then rstd (written; the backward pass reads it);
- * drop nullable; y may be x.  workspace: caller-owned, 16-byte aligned, of fisr_train_groupnorm_workspace_bytes (enough for any type, stride
+ * drop nullable; y may be x.  var + eps has to be at least 2^-126 (with eps = 0: a spread above 1e-19), where rstd is finite and
+ * the backward pass can square it.  workspace: caller-owned, 16-byte aligned, of fisr_train_groupnorm_workspace_bytes (enough for any type, stride
  * and alignment; 0: bad shape).  A forward call that needs none may be made without one: FISR_ENOMEM says where it does. */
 FISR_API size_t fisr_train_groupnorm_workspace_bytes(int n, int h, int w, int c, int groups, int backward);
 FISR_API int fisr_train_groupnorm(const void* x, int x_cs, const float* gamma, const float* beta, void* y, int y_cs, float* mean_rstd, int n,
