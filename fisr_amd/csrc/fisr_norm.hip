@@ -39,17 +39,16 @@ constexpr int MOST_WORKGROUPS = 2048;                          // of a batch, by
 
 // Workspace: `part` of n * chunks * c float2, and for the backward pass s12 of n * groups * chunks and ab of n * c.  Not a function of the
 // vector width or the form that runs: its size is asked for without the tensors.
-struct WsLayout { size_t part, s12, ab; };
+struct WsLayout {
+  size_t part, s12, ab;
+  size_t bytes() const { return (part + s12 + ab) * sizeof(float2); }
+};
 WsLayout ws_layout(const NormArgs& a, bool backward) {
   int chunks, ppc;
   chunks_for(a, MOST_WORKGROUPS, LEAST_ELEMENTS, chunks, ppc);
   WsLayout w{(size_t)a.n * chunks * a.c, 0, 0};
   if (backward) { w.s12 = (size_t)a.n * a.groups * chunks; w.ab = (size_t)a.n * a.c; }
   return w;
-}
-size_t norm_ws_bytes(const NormArgs& a, bool backward) {
-  const WsLayout w = ws_layout(a, backward);
-  return (w.part + w.s12 + w.ab) * sizeof(float2);
 }
 
 // Vectors of 16 bytes where all tensors allow such accesses, else of 8 and so on down to one channel.
@@ -241,25 +240,26 @@ const char* drop_error(const fisr_dropout* d, DropArgs& out) {
   if ((uintptr_t)d->d_counter % 8) return "dropout: d_counter is not aligned to 8 bytes";
   return nullptr;
 }
-// Where an operand lies: `count` runs of `run` bytes, `step` bytes from one to the next.
+// Where an operand lies: runs of `run` bytes, `step` bytes from one to the next, up to `end`; one run has run = step.
 struct Place {
-  uintptr_t at;
-  size_t run, step, count;
-  Place(const void* p, size_t bytes) : at((uintptr_t)p), run(bytes), step(bytes), count(1) {}
-  Place(const void* p, size_t pixels, size_t c, size_t cs, size_t elem_bytes) : at((uintptr_t)p), run(c * elem_bytes), step(cs * elem_bytes), count(pixels) {
-    if (run == step || count == 1) { run *= count; step = run; count = 1; }      // no gaps
+  uintptr_t at = 0, end = 0;
+  size_t run = 0, step = 0;
+  Place(const void* p, size_t bytes) {
+    if (p) { at = (uintptr_t)p; end = at + bytes; run = step = bytes; }
   }
-  uintptr_t end() const { return at + (count - 1) * step + run; }
-  bool same(const Place& o) const { return at == o.at && run == o.run && step == o.step && count == o.count; }
-  // Whether they share a byte (runs at two steps: taken to)
+  Place(const void* p, size_t pixels, size_t c, size_t cs, size_t elem_bytes) : Place(p, ((pixels - 1) * cs + c) * elem_bytes) {
+    if (p && pixels > 1 && cs != c) { run = c * elem_bytes; step = cs * elem_bytes; }
+  }
+  bool dense() const { return run == step; }
+  bool same(const Place& o) const { return at == o.at && end == o.end && run == o.run && step == o.step; }
+  // Whether they share a byte (runs at two steps whose ranges meet: taken to)
   bool meets(const Place& o) const {
-    if (!at || !o.at || !run || !o.run || end() <= o.at || o.end() <= at) return false;
-    if (count == 1 && o.count == 1) return true;
-    if (count > 1 && o.count > 1 && step != o.step) return true;
-    const size_t every = count > 1 ? step : o.step;
+    if (at >= o.end || o.at >= end || !run || !o.run) return false;
+    if (dense() && o.dense()) return true;
+    if (!dense() && !o.dense() && step != o.step) return true;
+    const size_t every = dense() ? o.step : step;
     const size_t from = at >= o.at ? (at - o.at) % every : (every - (o.at - at) % every) % every;      // where a run of this begins, after one of the other's
-    const size_t run_a = std::min(run, every), run_b = std::min(o.run, every);
-    return from < run_b || from + run_a > every;
+    return from < std::min(o.run, every) || from + std::min(run, every) > every;
   }
 };
 // The device that a call's operands are on, null ones aside; -1 where one is not memory of a GPU or of another one than those before it (every
@@ -304,8 +304,9 @@ int norm_call(const char* who, NormArgs& a, bool backward, int n, int h, int w, 
   a.mean = mean_rstd; a.rstd = mean_rstd + (size_t)n * groups;
   if ((uintptr_t)ws % 16) return bad("the workspace is not aligned to 16 bytes");
   a.team = team_variant(a, es == 4 ? norm_vec<float>(a) : norm_vec<f16_t>(a), (int)es, backward);
-  if ((backward || a.team < 0) && (!ws || ws_bytes < norm_ws_bytes(a, backward))) return set_error(FISR_ENOMEM, std::string(who) + ": workspace too small");
-  const WsLayout lay = ws_layout(a, backward);
+  const bool work = backward || a.team < 0;
+  const WsLayout lay = work ? ws_layout(a, backward) : WsLayout{};
+  if (work && (!ws || ws_bytes < lay.bytes())) return set_error(FISR_ENOMEM, std::string(who) + ": workspace too small");
   a.part = (float2*)ws;
   a.s12 = a.part + lay.part;
   a.ab = a.s12 + lay.s12;
@@ -314,7 +315,7 @@ int norm_call(const char* who, NormArgs& a, bool backward, int n, int h, int w, 
   const int dev = operands_device({{"gamma", READ, {a.gamma, params}}, {"beta", READ, {a.beta, params}}, {"dgamma", WRITTEN, {a.dgamma, params}},
                                    {"dbeta", WRITTEN, {a.dbeta, params}}, {"d_counter", READ, {a.drop.counter, sizeof(uint64_t)}},
                                    {"mean_rstd", backward ? READ : WRITTEN, {mean_rstd, 2 * sizeof(float) * n * groups}},
-                                   {"the workspace", WRITTEN, {ws, backward || a.team < 0 ? norm_ws_bytes(a, backward) : 0}},
+                                   {"the workspace", WRITTEN, {ws, lay.bytes()}},
                                    {"dy", IN_PLACE, {a.dy, pixels, (size_t)c, a.dycs, es}}, {"x", IN_PLACE, {a.x, pixels, (size_t)c, a.xcs, es}},
                                    {backward ? "dx" : "y", OUT, {a.y, pixels, (size_t)c, a.ycs, es}}}, error);
   if (dev < 0) return bad(error.c_str());
@@ -353,7 +354,7 @@ size_t fisr_train_groupnorm_workspace_bytes(int n, int h, int w, int c, int grou
   if (norm_shape_error(n, h, w, c, groups)) return 0;
   NormArgs a{};
   a.n = n; a.p = h * w; a.c = c; a.groups = groups;
-  return norm_ws_bytes(a, backward != 0);
+  return ws_layout(a, backward != 0).bytes();
 }
 
 int fisr_train_groupnorm(const void* x, int x_cs, const float* gamma, const float* beta, void* y, int y_cs, float* mean_rstd, int n, int h, int w,

@@ -205,9 +205,9 @@ def group_norm_backward(dy, x, stats, groups, gamma=None, beta=None, *, act="non
     code, dev = _type(x)
     _like(dy, x, dev, "dy")
     x_cs, dy_cs = _pixel_stride(x, "x"), _pixel_stride(dy, "dy")
-    given = dx, dgamma, dbeta
+    given = None if dx is None and dgamma is None and dbeta is None else (dx, dgamma, dbeta)
     dx, dx_cs = _out(x, dx, x_cs, dev, "dx")
-    if given[0] is not None and x.numel():
+    if given and given[0] is not None and x.numel():
         _apart(dx, dx_cs, dy, dy_cs, "dx")
         _apart(dx, dx_cs, x, x_cs, "dx")
     if accumulate and (dgamma is None or dbeta is None):
@@ -224,7 +224,8 @@ def group_norm_backward(dy, x, stats, groups, gamma=None, beta=None, *, act="non
                     ws.data_ptr(), nbytes, _stream(dev))
     if rc < 0:
         _lib.check(rc)
-    _wrote(*given)
+    if given:
+        _wrote(*given)
     return dx, dgamma, dbeta
 
 
