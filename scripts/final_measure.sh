@@ -1,8 +1,10 @@
 #!/bin/bash
-# The round's final measurement on ONE gpurun box (r06): the rocprofv3 trace + PMC passes per engine (scripts/gpu_profile.sh), their
-# tables installed under profiles/ ON THE BOX so that the bench lines of the same library read them, then the default bench line and
-# the `mixed` one with per-layer tables.  Everything lands in gpurun_out/final/; copy what should be kept into profiles/.
-#   gpurun --timeout 3000 -- 'bash scripts/final_measure.sh'
+# The counter tables and bench lines of a finished library on ONE box (about 5 minutes): the rocprofv3 trace + PMC passes per engine
+# (scripts/gpu_profile.sh), their tables installed under profiles/ ON THE BOX so that the bench lines of the same library read them, then the
+# default bench line and the `mixed` one with per-layer tables.  Everything lands in gpurun_out/final/; what is kept goes into profiles/.  bench.py
+# drops the tables of any other library than the one that runs, so this is run again after every change under csrc/ or of include/fisr.h.
+# The first step that fails ends the script.
+set -e
 REPO="${GRAFT_REPO_ROOT:-/root/repo}"
 F="$REPO/gpurun_out/final"
 mkdir -p "$F"
@@ -18,6 +20,6 @@ cp gpurun_out/prof_fp32/pmc_traffic.json profiles/pmc_traffic.json && cp profile
 cp gpurun_out/prof_fp32/summary.txt "$F/rocprofv3_all_engines_summary.txt"
 rm -rf gpurun_out/prof_fp32
 cd /tmp
-timeout 900 python "$REPO/bench.py" --layer-profile "$F/layers_fp32.json" > "$F/bench_default.json" 2> "$F/bench_default.err"; echo "bench default rc=$?"
-timeout 600 python "$REPO/bench.py" --precision mixed --others none --no-cpu-baseline --no-train --layer-profile "$F/layers_mixed.json" > "$F/bench_mixed.json" 2> "$F/bench_mixed.err"; echo "bench mixed rc=$?"
+timeout 900 python "$REPO/bench.py" --layer-profile "$F/layers_fp32.json" > "$F/bench_default.json" 2> "$F/bench_default.err"
+timeout 600 python "$REPO/bench.py" --precision mixed --others none --no-cpu-baseline --no-train --layer-profile "$F/layers_mixed.json" > "$F/bench_mixed.json" 2> "$F/bench_mixed.err"
 tail -c 1500 "$F/bench_default.json"

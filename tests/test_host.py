@@ -388,3 +388,21 @@ def test_committed_pmc_tables_hold_no_impossible_clock():
                 assert e.get("cycle_columns_nulled") and e.get("mfma_busy_frac") is None, (f, k)
             else:
                 assert 500.0 <= clk <= 2500.0, (f, k, clk)
+
+
+@pytest.mark.parametrize("engine,kernel", [("fp32", "conv3x3_wf4<f32w4,relu_in,nores>"), ("mixed", "conv3x3_dma<f16>"), ("f16f8", "conv3x3_dma_fs<f16f8,tw32,relu_in,nores>"),
+                                           (None, "conv3x3_wf4<f32w4,relu_in,nores>")])
+def test_counter_tables_are_of_this_tree(engine, kernel):
+    """The committed counter tables are of one library, and bench.py takes each engine's dominant kernel from them.  They are of these sources:
+    after a change of the library it drops them until they are made again, which this test says by skipping."""
+    import bench_report as b
+    from fisr_amd import lib
+    tables = {e: b._pmc_table(e)["_meta"]["library"] for e in ("fp32", "mixed", "f16f8", None)}
+    assert len({b._src_of(v) for v in tables.values()}) == 1, tables
+    running = "fisr_hip 0.3 (gfx950) src " + lib.source_hash()
+    if b._src_of(tables[engine]) != lib.source_hash():
+        assert b._pmc_table_checked(running, engine)[0] == {}
+        pytest.skip(f"the tables are of {tables[engine]}, the sources are {running}: make them again with scripts/final_measure.sh")
+    table, _ = b._pmc_table_checked(running, engine)
+    key = next(k for k in table if k.startswith(b._pmc_key(kernel)))
+    assert table[key]["hbm_bytes_per_launch"] > 0 and 0 < table[key]["mfma_busy_frac"] < 1
