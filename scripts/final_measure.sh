@@ -1,6 +1,6 @@
 #!/bin/bash
-# The counter tables and bench lines of a finished library on ONE box (about 5 minutes): the rocprofv3 trace + PMC passes per engine
-# (scripts/gpu_profile.sh), their tables installed under profiles/ ON THE BOX so that the bench lines of the same library read them, then the
+# The counter tables and bench lines of a finished library on ONE machine (about 3 minutes): the rocprofv3 trace + PMC passes per engine
+# (scripts/gpu_profile.sh), their tables installed under profiles/ THERE so that the bench lines of the same library read them, then the
 # default bench line and the `mixed` one with per-layer tables.  Everything lands in gpurun_out/final/; what is kept goes into profiles/.  bench.py
 # drops the tables of any other library than the one that runs, so this is run again after every change under csrc/ or of include/fisr.h.
 # The first step that fails ends the script.
